@@ -44,6 +44,7 @@ SIGNATURES = {
     "cmx_rt_stream_sync": (i32, [vp]),
     "cmx_mx_quant": (i32, [vp, u32, u8p, u32, u8p, u32, u32, u32, i32, i32, vp]),
     "cmx_mx_dequant": (i32, [u8p, u32, u8p, u32, f32p, u32, u32, u32, i32, vp]),
+    "cmx_rms_norm_quant": (i32, [vp, u32, vp, u32, vp, vp, u32, vp, u32, u8p, u32, u8p, u32, u32, u32, u32, i32, i32, i32, vp]),
     "cmx_mx_gemm": (i32, [u8p, u32, u8p, u32, u8p, u32, u8p, u32, vp, u32, u32, u32, u32, i32, i32, vp]),
     "cmx_mx_gmm_workspace_bytes": (sz, [u32]),
     "cmx_mx_gmm": (i32, [u8p, u32, u8p, u32, u8p, u8p, vp, u32, i32p, u32, u32, u32, u32, i32, i32, vp, vp]),

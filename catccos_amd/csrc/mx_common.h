@@ -46,6 +46,7 @@ void set_error(const std::string& msg);
 int preload_routing_kernels();
 int preload_layout_kernels();
 int preload_quant_kernels();
+int preload_norm_kernels();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }

@@ -8,6 +8,7 @@ anything in torch.
 """
 from __future__ import annotations
 
+import struct
 from operator import index
 
 import torch
@@ -43,6 +44,7 @@ _FP4 = ("E2M1", "E1M2")
 ROUND = {"rne": 0, "lut": 1}
 OUT = {"bf16": 0, "fp16": 1, "fp32": 2}
 _OUT_DTYPE = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+_TYPE = {torch.bfloat16: 0, torch.int16: 0, torch.uint16: 0, torch.float16: 1, torch.float32: 2}
 
 
 # not a public function of torch, so it may be missing
@@ -90,6 +92,36 @@ def _need_cuda(*ts):
             raise ValueError("expected a GPU tensor")
 
 
+def _here(*ts):
+    """GPU tensors (or Nones) of the device that torch's current stream is on, or ValueError: a kernel launched on another device could not reach them."""
+    device = None
+    for t in ts:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"expected a tensor, not {type(t).__name__}")
+        at = t.get_device()
+        if at < 0:
+            raise ValueError("expected a GPU tensor")
+        if device is None:
+            device = _device()
+        if at != device:
+            raise ValueError(f"expected tensors on the current device ({device}), not on device {at}")
+
+
+def _pitch(t) -> int:
+    """Elements from row to row of a 2-D tensor whose rows lie in one piece (what torch gives a single row as its stride says nothing)."""
+    rows, cols = t.shape
+    pitch, step = t.stride()
+    assert step == 1 or cols <= 1, "rows must lie in one piece"
+    return pitch if rows > 1 else cols
+
+
+def _bits(value) -> int:
+    """A number as the 32 bits of a float: the entry points take integers and pointers only."""
+    return struct.unpack("I", struct.pack("f", value))[0]
+
+
 def scale_cols(cols: int) -> int:
     nb = (cols + 31) // 32
     return (nb + 1) // 2 * 2
@@ -117,6 +149,48 @@ def mx_dequant(codes: torch.Tensor, scales: torch.Tensor, cols: int, fmt: str = 
     _lib.check(lib.cmx_mx_dequant(_p(codes), codes.stride(0), _p(scales), scales.stride(0), _p(out), cols, rows, cols,
                                   FMT[fmt], _stream()))
     return out
+
+
+def _norm(x, weight, eps, residual, total, y, codes, scales, code_cols, fmt):
+    """cmx_rms_norm_quant; y, codes and scales: a new tensor's dtype and sizes, or None.  Returns the new tensors and the total."""
+    _here(x, weight, residual, total)
+    rows, cols = x.shape
+    assert weight.shape == (cols,) and weight.is_contiguous() and (weight.dtype == x.dtype or weight.dtype == torch.float32)
+    r_pitch = t_pitch = cols
+    into = total
+    if residual is None:
+        assert total is None, "a total needs a residual"
+    else:
+        assert residual.shape == x.shape and residual.dtype == x.dtype
+        r_pitch = _pitch(residual)
+        if total is None:
+            into = (x.dtype, rows, cols)
+        else:
+            assert total.shape == x.shape and total.dtype == x.dtype
+            t_pitch = _pitch(total)
+    made = _launch("cmx_rms_norm_quant", x, _pitch(x), residual, r_pitch, weight, into, t_pitch, y, cols, codes, code_cols, scales,
+                   0 if scales is None else scales[2], rows, cols, _bits(eps), _TYPE[x.dtype], _TYPE[weight.dtype], FMT[fmt])
+    made = list(made) if made.__class__ is tuple else [made]
+    return made, made.pop(0) if into is not total else total
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual=None, total=None):
+    """x [rows, cols] bf16 / fp16 / fp32, weight [cols] of x's type or fp32 -> (y, t): t = x + residual and y = t / rms(t) * weight, computed in fp32
+    and rounded once to x's type.  t is None without a residual; with one it is a new tensor, or `total`, which may be x or the residual."""
+    rows, cols = x.shape
+    (y,), total = _norm(x, weight, eps, residual, total, (x.dtype, rows, cols), None, None, 0, "E4M3")
+    return y, total
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual=None, fmt: str = "E4M3", want_y: bool = False, total=None):
+    """rms_norm straight to MX codes, E4M3, E5M2 or E2M1 to nearest-even: (codes, scales, y|None, t|None), codes and scales as mx_quant gives them but
+    made of y before it is rounded."""
+    rows, cols = x.shape
+    code_cols = (cols + 1) // 2 if fmt in _FP4 else cols
+    made, total = _norm(x, weight, eps, residual, total, (x.dtype, rows, cols) if want_y else None, (torch.uint8, rows, code_cols),
+                        (torch.uint8, rows, scale_cols(cols)), code_cols, fmt)
+    codes, scales = made[-2:]
+    return codes, scales, made[0] if want_y else None, total
 
 
 def mx_gemm(a, a_scale, b, b_scale, k: int, fmt: str = "E4M3", out: str = "bf16") -> torch.Tensor:

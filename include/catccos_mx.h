@@ -99,6 +99,29 @@ int cmx_mx_dequant(const uint8_t* codes, uint32_t ld_codes, const uint8_t* scale
                    uint32_t ld_out, uint32_t rows, uint32_t cols, int fmt, cmx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Root-mean-square norm with the residual's addition, to 16 or 32 bits and / or to MX codes: what stands in front of a
+ * matmul, the gate or the experts of a layer (no counterpart in the reference, whose operators start at the activations).
+ *   t = x + residual;   y = t / sqrt(mean(t^2) + eps) * weight
+ * in fp32, from any input type; total receives t and y_out y, each rounded once to the type of x; codes and scales are those of
+ * y before that rounding, nearest-even, by the rules and in the layout of cmx_mx_quant (padding column and non-finite blocks
+ * among them).
+ *
+ *   x         [rows, cols] of `type` (CMX_OUT_BF16 / FP16 / FP32), pitch ld_x elements
+ *   residual  the same, or NULL: t = x
+ *   weight    [cols] of weight_type: `type` or CMX_OUT_FP32
+ *   total     [rows, cols] of `type`, or NULL; needs a residual.  May be x or residual themselves (same pointer and pitch); no
+ *             other overlap of inputs and outputs
+ *   y_out     [rows, cols] of `type`, or NULL
+ *   codes     u8, E4M3 / E5M2 / E2M1 by fmt, with scales; both or neither.  y_out or codes must be given
+ *   eps_bits  eps as the 32 bits of a float (every argument of this interface is an integer or a pointer); >= 0
+ * Rows need only their elements' alignment.  A row whose squares overflow fp32 gives zeros, as 1 / sqrt(inf) says.
+ * ---------------------------------------------------------------------------------------- */
+int cmx_rms_norm_quant(const void* x, uint32_t ld_x, const void* residual, uint32_t ld_residual, const void* weight,
+                       void* total, uint32_t ld_total, void* y_out, uint32_t ld_y, uint8_t* codes, uint32_t ld_codes,
+                       uint8_t* scales, uint32_t ld_scales, uint32_t rows, uint32_t cols, uint32_t eps_bits, int type,
+                       int weight_type, int fmt, cmx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Dense MX matmul  C[m,n] = sum_k deq(A)[m,k] * deq(B)[n,k]   (both operands K-contiguous).
  * Replaces the AIC loop of MatmulReduceScatterMxTla
  * (include/catccos/dgemm/kernel/matmul_reduce_scatter_mx_tla.hpp:190-315: blockMmad(A,B,C,shape,
