@@ -42,6 +42,7 @@ def _empty(*args):
 FMT = {"E4M3": 0, "E5M2": 1, "E2M1": 2, "E1M2": 3}
 _FP4 = ("E2M1", "E1M2")
 ROUND = {"rne": 0, "lut": 1}
+SCORE = {"softmax": 0, "sigmoid": 1}
 OUT = {"bf16": 0, "fp16": 1, "fp32": 2}
 _OUT_DTYPE = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 _TYPE = {torch.bfloat16: 0, torch.int16: 0, torch.uint16: 0, torch.float16: 1, torch.float32: 2}
@@ -372,6 +373,19 @@ def mx_gmm_swiglu_quant_noalloc(a, a_scale, b, b_scale, group_sizes, k: int, cod
 def init() -> None:
     """cmx_init on the current device."""
     _lib.check(_lib.load().cmx_init())
+
+
+def moe_gating(logits: torch.Tensor, top_k: int, score: str = "softmax", bias=None, groups: int = 1, top_groups: int = 1, group_best: int = 1,
+               renormalize: bool = True, scale: float = 1.0):
+    """logits [T, experts] bf16 / fp16 / fp32 -> (expert_idx int32, gate_weight fp32) [T, top_k], as moe_init_routing and dispatch_ffn_combine take them.
+    The top_k largest scores + bias (fp32 [experts]) in falling order, from the top_groups of `groups` groups of neighbours whose group_best (1 or 2) largest
+    have the largest sum; ties to the lower index.  The weights are the scores without the bias, over their sum if renormalize, times scale."""
+    top_k, groups, top_groups, group_best = index(top_k), index(groups), index(top_groups), index(group_best)
+    _here(logits, bias)
+    tokens, experts = logits.shape
+    assert bias is None or (bias.shape == (experts,) and bias.dtype == torch.float32 and bias.is_contiguous())
+    return _launch("cmx_moe_gating", logits, _pitch(logits), _TYPE[logits.dtype], bias, tokens, experts, top_k, SCORE[score], groups, top_groups, group_best,
+                   1 if renormalize else 0, _bits(scale), (torch.int32, tokens, top_k), (torch.float32, tokens, top_k))
 
 
 def moe_init_routing(expert_idx: torch.Tensor, experts: int):

@@ -40,6 +40,10 @@ extern "C" {
 #define CMX_OUT_FP16 1
 #define CMX_OUT_FP32 2
 
+/* scores of the gate */
+#define CMX_SCORE_SOFTMAX 0
+#define CMX_SCORE_SIGMOID 1
+
 typedef void* cmx_stream_t;
 
 int cmx_version(void);
@@ -310,6 +314,28 @@ int cmx_int8_gmm_dequant_swiglu(const int8_t* a, uint32_t lda, const float* toke
                                 const float* channel_scale, uint32_t channel_scale_stride, void* out, uint32_t ld_out,
                                 int out_type, const int32_t* group_sizes, uint32_t groups, uint32_t m_total, uint32_t n,
                                 uint32_t k, int trans_b, void* workspace, cmx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The gate of an MoE layer: from logits to the expert_idx and gate_weight that cmx_moe_init_routing and the FFN take (no
+ * counterpart in the reference, whose operators start at the chosen experts).
+ *   s = softmax(logits) or sigmoid(logits) by `score`;  c = s + bias
+ *   kept groups: the top_groups of `groups` groups of experts / groups neighbours whose group_best (1 or 2) largest c have the
+ *   largest sum;  chosen: the top_k largest c in them, in falling order;  gate_weight = s * scale, with renormalize over
+ *   the sum of the chosen s first (zero if that is zero).  Ties go to the lower index, for groups too.
+ * The order is that of the exact values, not of values rounded to fp32: without a bias and with one value for each group logits are compared, elsewhere
+ * c in up to 64 bits.
+ *
+ *   logits       [tokens, experts] of `type` (CMX_OUT_BF16 / FP16 / FP32), pitch ld_logits elements
+ *   bias         fp32 [experts] or NULL; it moves the choice, not the weights
+ *   scale_bits   scale as the 32 bits of a float
+ *   expert_idx   int32 [tokens, top_k], gate_weight fp32 [tokens, top_k]
+ * experts <= 1024, groups <= 64 and a divisor of experts, top_k <= 64.  A logit or bias of -Inf masks an expert: it is chosen
+ * when no other is left.  A row of -Inf has scores of zero.  NaN ranks behind -Inf; a NaN or +Inf in a softmax row makes
+ * its weights NaN.  Whatever a row holds, its indices are distinct and in [0, experts).
+ * ---------------------------------------------------------------------------------------- */
+int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, const float* bias, uint32_t tokens, uint32_t experts,
+                   uint32_t top_k, int score, uint32_t groups, uint32_t top_groups, uint32_t group_best, int renormalize,
+                   uint32_t scale_bits, int32_t* expert_idx, float* gate_weight, cmx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * MoE routing: stable sort of (expert, row) pairs.

@@ -1,0 +1,197 @@
+"""The gate against the definition in 64 bits: the same indices, and weights to what fp32 leaves of them."""
+import math
+
+import pytest
+import torch
+
+from catccos_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+# Relative error of a weight in fp32.  Softmax: |z - max| * 2^-24 from the difference (|z| stays below 10 here, so at most 20), exp 2 units, 16 + 6
+# additions, and the same for the sum that divides it, a division and the scale: (20 + 2 + 22 + 2) * 2 * 2^-24 < 2^-17
+WEIGHT_LOSS = 2.0 ** -17
+
+
+def _definition(z, top_k, score, bias, groups, top_groups, group_best, renormalize, scale):
+    z = z.double()
+    if score == "softmax":
+        most = z.amax(dim=1, keepdim=True)
+        s = torch.where(z == -math.inf, 0.0, torch.exp(z - most))
+        total = s.sum(dim=1, keepdim=True)
+        s = torch.where(total == 0, 0.0, s / total)
+    else:
+        s = 1 / (1 + torch.exp(-z))
+    c = s if bias is None else s + bias.double()
+    t, e = z.shape
+    if groups > 1:
+        c = c.view(t, groups, -1)
+        best = c.sort(dim=2, descending=True).values[:, :, :group_best].sum(dim=2)
+        kept = best.sort(dim=1, descending=True, stable=True).indices[:, :top_groups]
+        closed = torch.ones_like(best, dtype=torch.bool).scatter(1, kept, False)
+        order = torch.where(closed[:, :, None].expand_as(c), 1, 0).reshape(t, e)
+        c = c.reshape(t, e)
+        by_value = c.sort(dim=1, descending=True, stable=True).indices
+        idx = by_value.gather(1, order.gather(1, by_value).sort(dim=1, stable=True).indices)[:, :top_k]      # closed groups behind the open ones
+    else:
+        idx = c.sort(dim=1, descending=True, stable=True).indices[:, :top_k]
+    w = s.gather(1, idx)
+    if renormalize:
+        total = w.sum(dim=1, keepdim=True)
+        w = torch.where(total == 0, 0.0, w / total)
+    return idx, w * scale
+
+
+def _check(z, top_k, score="softmax", bias=None, groups=1, top_groups=1, group_best=1, renormalize=True, scale=1.0):
+    idx, w = ops.moe_gating(z, top_k, score, bias, groups, top_groups, group_best, renormalize, scale)
+    want_idx, want_w = _definition(z, top_k, score, bias, groups, top_groups, group_best, renormalize, scale)
+    assert idx.dtype == torch.int32 and w.dtype == torch.float32 and idx.shape == w.shape == (z.shape[0], top_k)
+    rows = (idx.long() != want_idx).any(dim=1).nonzero().flatten().tolist()
+    assert not rows, f"{len(rows)} rows differ, the first: {rows[0]}: {idx[rows[0]].tolist()} for {want_idx[rows[0]].tolist()}"
+    err = (w.double() - want_w).abs()
+    assert bool((err <= want_w.abs() * WEIGHT_LOSS + 2.0 ** -140).all()), float((err / want_w.abs().clamp_min(1e-300)).max())
+
+
+def _logits(tokens, experts, dtype, seed, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (std * torch.randn((tokens, experts), generator=g, device="cuda")).to(DTYPES[dtype]), 0.05 * torch.randn(experts, generator=g, device="cuda")
+
+
+SIZES = [(1, 1), (2, 2), (8, 1), (8, 8), (16, 4), (17, 3), (32, 32), (33, 5), (64, 6), (100, 10), (128, 64), (160, 7), (255, 9), (256, 8), (257, 8), (384, 64),
+         (512, 16), (1000, 12), (1024, 64)]
+
+
+@pytest.mark.parametrize("experts,top_k", SIZES)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_every_size(experts, top_k, dtype):
+    for tokens in (1, 5, 67, 2051):
+        z, bias = _logits(tokens, experts, dtype, experts + tokens)
+        for score in ("softmax", "sigmoid"):
+            for b in (None, bias):
+                _check(z, top_k, score, b, renormalize=tokens != 67, scale=2.5 if tokens == 5 else 1.0)
+
+
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [(8, 2, 1, 4), (8, 8, 3, 3), (16, 4, 2, 5), (24, 3, 2, 9), (60, 20, 7, 6), (64, 64, 10, 10), (256, 8, 4, 8),
+                                                              (256, 16, 3, 30), (320, 64, 9, 33), (512, 32, 32, 64), (1000, 10, 2, 8), (1024, 16, 5, 64)])
+@pytest.mark.parametrize("group_best", [1, 2])
+def test_groups(experts, groups, top_groups, top_k, group_best):
+    for tokens, dtype in ((1, "fp32"), (7, "bf16"), (2100, "fp32"), (2100, "bf16")):
+        z, bias = _logits(tokens, experts, dtype, experts + tokens + group_best)
+        for score in ("softmax", "sigmoid"):
+            for b in (None, bias):
+                _check(z, top_k, score, b, groups, top_groups, group_best, renormalize=tokens != 7)
+
+
+@pytest.mark.parametrize("tokens", [3, 3000])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_ties_go_to_the_lower_index(tokens, score):
+    for levels in (1, 2, 5):                                           # few different values: nearly everything ties
+        g = torch.Generator(device="cuda").manual_seed(levels)
+        z = torch.randint(0, levels, (tokens, 256), generator=g, device="cuda").float()
+        for bias in (None, torch.zeros(256, device="cuda"), torch.randint(0, 2, (256,), generator=g, device="cuda").float()):
+            _check(z, 8, score, bias)
+            _check(z, 8, score, bias, 8, 4, 2)
+            _check(z, 8, score, bias, 8, 4, 1)
+
+
+@pytest.mark.parametrize("tokens", [16, 4096])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_values_that_fp32_cannot_tell_apart(tokens, score):
+    """Logits that differ in their last bit only, and biases that make up for differences in the score to about the last bit of fp32: the order is still
+    that of 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    base = torch.randn((tokens, 1), generator=g, device="cuda")
+    step = torch.randint(-3, 4, (tokens, 256), generator=g, device="cuda", dtype=torch.int32)
+    z = (base.expand(tokens, 256).contiguous().view(torch.int32) + step).view(torch.float32)
+    _check(z, 8, score)
+    _check(z, 8, score, torch.zeros(256, device="cuda"))
+    _check(z, 8, score, torch.zeros(256, device="cuda"), 8, 4, 2)
+    z = torch.randn((1, 256), generator=g, device="cuda").expand(tokens, 256).contiguous()
+    s = torch.softmax(z[:1].double(), dim=1) if score == "softmax" else torch.sigmoid(z[:1].double())
+    _check(z, 8, score, (0.75 - s[0]).float())
+    _check(z, 8, score, (0.75 - s[0]).float(), 16, 4, 2)
+    _check(z * 30, 8, score, torch.zeros(256, device="cuda"))           # sigmoids that fp32 rounds to one, exps that it loses
+
+
+def test_masked_experts_and_rows_without_any():
+    tokens, experts = 2500, 96
+    z, bias = _logits(tokens, experts, "fp32", 4)
+    z[:, 10:] = torch.where(torch.rand((tokens, experts - 10), device="cuda") < 0.9, -math.inf, z[:, 10:])
+    z[7] = -math.inf
+    z[8, 1:] = -math.inf
+    z[9] = torch.finfo(torch.float32).min
+    for score in ("softmax", "sigmoid"):
+        for b in (None, bias, torch.where(torch.arange(experts, device="cuda") % 3 == 0, -math.inf, bias)):
+            for part in (z, z[5:12]):
+                _check(part, 16, score, b)
+                _check(part, 16, score, b, 8, 4, 1)
+    w = ops.moe_gating(z[7:8], 4)[1]
+    assert bool((w == 0).all())
+
+
+@pytest.mark.parametrize("tokens", [40, 2500])
+def test_indices_stay_distinct_and_in_range_whatever_a_row_holds(tokens):
+    g = torch.Generator(device="cuda").manual_seed(8)
+    z = torch.randn((tokens, 256), generator=g, device="cuda")
+    z = torch.where(torch.rand(z.shape, generator=g, device="cuda") < 0.6, math.nan, z)
+    z = torch.where(torch.rand(z.shape, generator=g, device="cuda") < 0.1, math.inf, z)
+    z[3] = math.nan
+    z[4] = math.inf
+    for score in ("softmax", "sigmoid"):
+        for b in (None, torch.where(torch.arange(256, device="cuda") < 100, math.nan, 0.1), torch.full((256,), math.inf, device="cuda")):
+            for args in ((1, 1, 1), (8, 4, 2), (8, 2, 1)):
+                idx, w = ops.moe_gating(z, 32, score, b, *args)
+                s = idx.long().sort(dim=1).values
+                assert bool((s[:, 0] >= 0).all()) and bool((s[:, -1] < 256).all()) and bool((s[:, 1:] > s[:, :-1]).all())
+                if score == "softmax":
+                    assert bool(w.isnan().all())                        # every row here holds a NaN or +Inf
+    # a NaN ranks behind the others
+    z = torch.zeros((tokens, 64), device="cuda")
+    z[:, ::2] = math.nan
+    idx, _ = ops.moe_gating(z, 40, "sigmoid")
+    assert bool((idx[:, :32] == torch.arange(1, 64, 2, device="cuda")).all()) and bool((idx[:, 32:] == torch.arange(0, 16, 2, device="cuda")).all())
+
+
+def test_strided_rows_past_32_bits_and_no_rows():
+    z, bias = _logits(9, 300, "bf16", 3)
+    view = z[::2, 7:263]
+    assert all(torch.equal(p, q) for p, q in zip(ops.moe_gating(view, 8), ops.moe_gating(view.contiguous(), 8)))
+    apart = (1 << 32) - 8
+    buf = torch.empty(apart + 256, dtype=torch.bfloat16, device="cuda")
+    far = buf.as_strided((2, 256), (apart, 1))
+    far.copy_(z[:2, :256])
+    assert all(torch.equal(p, q) for p, q in zip(ops.moe_gating(far, 8, "sigmoid", bias[:256], 8, 4, 2), ops.moe_gating(z[:2, :256], 8, "sigmoid", bias[:256], 8, 4, 2)))
+    idx, w = ops.moe_gating(z[:0], 8)
+    assert idx.shape == w.shape == (0, 8)
+
+
+def test_on_a_side_stream_and_captured():
+    ops.init()
+    z, bias = _logits(2100, 256, "fp32", 6)
+    call = lambda: ops.moe_gating(z, 8, "sigmoid", bias, 8, 4, 2, scale=2.5)
+    want = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for rep in range(3):
+        z.copy_(torch.randn(z.shape, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, call())), rep
+
+
+def test_into_the_routing_sort():
+    """The gate's answer is what moe_init_routing takes."""
+    z, _ = _logits(777, 256, "bf16", 2)
+    idx, w = ops.moe_gating(z, 8)
+    order, place, counts = ops.moe_init_routing(idx, 256)
+    assert torch.equal(counts.long(), torch.bincount(idx.flatten().long(), minlength=256))
+    assert torch.equal(order.long(), idx.flatten().long().sort(stable=True).indices)
+    assert bool(((w.sum(dim=1) - 1).abs() < 1e-5).all())
