@@ -46,6 +46,7 @@ SIGNATURES = {
     "cmx_mx_dequant": (i32, [u8p, u32, u8p, u32, f32p, u32, u32, u32, i32, vp]),
     "cmx_rms_norm_quant": (i32, [vp, u32, vp, u32, vp, vp, u32, vp, u32, u8p, u32, u8p, u32, u32, u32, u32, i32, i32, i32, vp]),
     "cmx_mx_gemm": (i32, [u8p, u32, u8p, u32, u8p, u32, u8p, u32, vp, u32, u32, u32, u32, i32, i32, vp]),
+    "cmx_mxfp4_gemv": (i32, [vp, u32, i32, u8p, u32, u8p, u32, vp, u32, i32, u32, u32, u32, vp]),
     "cmx_mx_gmm_workspace_bytes": (sz, [u32]),
     "cmx_mx_gmm": (i32, [u8p, u32, u8p, u32, u8p, u8p, vp, u32, i32p, u32, u32, u32, u32, i32, i32, vp, vp]),
     "cmx_mx_gmm_swiglu_quant": (i32, [u8p, u32, u8p, u32, u8p, u8p, u8p, u32, u8p, u32, vp, i32p, u32, u32, u32, u32,

@@ -1,0 +1,122 @@
+// out[m, n] = x[m, k] . deq(b)[n, k]^T for few rows of x: a matrix-vector product and a little more, bound by reading the weights once.
+//
+// A workgroup owns RT x 16 weight rows over the whole of K, which its wavefronts share out unit by unit; their sums meet in LDS.
+#include "mxfp4_rows.h"
+
+namespace cmx {
+namespace {
+
+struct GemvArgs {
+    const uint8_t *x, *b, *b_scale;
+    uint8_t* out;
+    size_t ld_x, ld_b, ld_scale, ld_out;      // bytes
+    uint32_t m, n, blocks;
+    int out_type;
+};
+
+// four consecutive results, or as many as `left`, to p
+__device__ __forceinline__ void store4(uint8_t* p, const v4f v, int type, uint32_t left) {
+    uint32_t w[4];
+    if (type == CMX_OUT_FP32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
+        if (left >= 4) __builtin_memcpy(p, w, 16);
+        else
+            for (uint32_t i = 0; i < left; ++i) reinterpret_cast<float*>(p)[i] = v[i];
+        return;
+    }
+    if (type == CMX_OUT_BF16) {
+        w[0] = cvt_pk_bf16(v[0], v[1]);
+        w[1] = cvt_pk_bf16(v[2], v[3]);
+    } else {
+        typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
+        w[0] = __builtin_bit_cast(uint32_t, (v2f16){(_Float16)v[0], (_Float16)v[1]});
+        w[1] = __builtin_bit_cast(uint32_t, (v2f16){(_Float16)v[2], (_Float16)v[3]});
+    }
+    if (left >= 4) {
+        __builtin_memcpy(p, w, 8);
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 3; ++i)
+        if (i < left) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+}
+
+template <int KIND, int RT, int CT, int UNIT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void mxfp4_gemv_kernel(const GemvArgs a) {
+    extern __shared__ v4f sums[];                                     // [wavefront][row tile][column tile][lane]
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const uint32_t row0 = blockIdx.x * (16 * RT), col0 = blockIdx.y * (16 * CT);
+    RowsTile<KIND, RT, CT, UNIT> t;
+    t.blocks = a.blocks;
+    t.plane = 0;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {                                    // rows past the last repeat it, and are not stored
+        const uint32_t row = min(row0 + i * 16 + (lane & 15), a.n - 1);
+        t.a[i] = a.b + row * a.ld_b + (lane >> 4) * 16;
+        t.scale[i] = a.b_scale + row * a.ld_scale + (lane >> 4);
+    }
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+        const uint32_t col = min(col0 + j * 16 + (lane & 15), a.m - 1);
+        t.x[j] = a.x + col * a.ld_x + (size_t)(lane >> 4) * 32 * XRegs<KIND>::kBytes;
+    }
+    t.clear();
+    t.run(wave, (a.blocks + 4 * UNIT - 1) / (4 * UNIT), waves);
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) sums[((wave * RT + i) * CT + j) * 64 + lane] = t.acc[i][j];
+    __syncthreads();
+    for (uint32_t at = threadIdx.x; at < RT * CT * 64; at += blockDim.x) {
+        v4f v = sums[at];
+        for (uint32_t w = 1; w < waves; ++w) v += sums[w * (RT * CT * 64) + at];
+        const uint32_t l = at & 63, i = (at >> 6) / CT, j = (at >> 6) % CT;
+        const uint32_t row = row0 + i * 16 + (l >> 4) * 4, col = col0 + j * 16 + (l & 15);     // of weights: output columns; of x: output rows
+        if (row < a.n && col < a.m)
+            store4(a.out + col * a.ld_out + (size_t)row * (a.out_type == CMX_OUT_FP32 ? 4 : 2), v, a.out_type, a.n - row);
+    }
+}
+
+template <int KIND>
+void launch(const GemvArgs& a, hipStream_t s) {
+    // `most` wavefronts, or as many as there are units of K
+    const auto run = [&](auto kernel, uint32_t rt, uint32_t ct, uint32_t unit, uint32_t most) {
+        const uint32_t units = ceil_div(a.blocks, 4 * unit), waves = units < most ? units : most;
+        hipLaunchKernelGGL(kernel, dim3(ceil_div(a.n, 16 * rt), ceil_div(a.m, 16 * ct)), dim3(64 * waves), waves * rt * ct * 1024, s, a);
+    };
+    if (a.m <= 16) run(mxfp4_gemv_kernel<KIND, 1, 1, 1, 16>, 1, 1, 1, 16);
+    else run(mxfp4_gemv_kernel<KIND, 2, 2, 1, 8>, 2, 2, 1, 8);
+}
+
+}  // namespace
+}  // namespace cmx
+
+int cmx::preload_gemv_kernels() {
+    hipFuncAttributes attr;
+    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::mxfp4_gemv_kernel<kXBf16, 1, 1, 1, 16>)));
+    return CMX_OK;
+}
+
+extern "C" int cmx_mxfp4_gemv(const void* x, uint32_t ld_x, int x_type, const uint8_t* b, uint32_t ld_b, const uint8_t* b_scale, uint32_t ld_bs,
+                              void* out, uint32_t ld_out, int out_type, uint32_t m, uint32_t n, uint32_t k, cmx_stream_t stream) {
+    using namespace cmx;
+    const auto known = [](int t) { return t == CMX_OUT_BF16 || t == CMX_OUT_FP16 || t == CMX_OUT_FP32; };
+    CMX_REQUIRE(known(x_type) && known(out_type), "unknown type");
+    if (m == 0 || n == 0) return CMX_OK;
+    CMX_REQUIRE(x && b && b_scale && out, "null pointer");
+    CMX_REQUIRE(k > 0 && k % 32 == 0, "k must be a positive multiple of 32");
+    CMX_REQUIRE(ld_x >= k && ld_b >= k / 2 && ld_bs >= k / 32 && ld_out >= n, "row pitch smaller than row");
+    CMX_REQUIRE(aligned16(b) && ld_b % 16 == 0, "weight rows must be 16-byte aligned");
+    const uint32_t xb = x_type == CMX_OUT_FP32 ? 4 : 2, ob = out_type == CMX_OUT_FP32 ? 4 : 2;
+    CMX_REQUIRE(reinterpret_cast<uintptr_t>(x) % xb == 0 && reinterpret_cast<uintptr_t>(out) % ob == 0, "pointers must be aligned to their elements");
+    CMX_REQUIRE(ceil_div(m, 16) <= 65535u, "too many rows of x");
+    const GemvArgs a = {static_cast<const uint8_t*>(x), b, b_scale, static_cast<uint8_t*>(out), (size_t)ld_x * xb, ld_b, ld_bs, (size_t)ld_out * ob, m, n, k / 32,
+                        out_type};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (x_type == CMX_OUT_BF16) launch<kXBf16>(a, s);
+    else if (x_type == CMX_OUT_FP16) launch<kXFp16>(a, s);
+    else launch<kXFp32>(a, s);
+    CMX_LAUNCH_CHECK();
+    return CMX_OK;
+}

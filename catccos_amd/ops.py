@@ -202,6 +202,14 @@ def mx_gemm(a, a_scale, b, b_scale, k: int, fmt: str = "E4M3", out: str = "bf16"
                    m, n, k, FMT[fmt], OUT[out])
 
 
+def mxfp4_gemv(x: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: str = "bf16") -> torch.Tensor:
+    """A few rows x [m, k] bf16 / fp16 / fp32, as they are, times MXFP4 weights b u8 [n, k/2] with b_scale u8 [n, >= k/32] -> [m, n]."""
+    _here(x, b, b_scale)
+    (m, k), n = x.shape, b.shape[0]
+    assert b.dtype == b_scale.dtype == torch.uint8 and 2 * b.shape[1] == k and b_scale.shape[0] == n and 32 * b_scale.shape[1] >= k
+    return _launch("cmx_mxfp4_gemv", x, _pitch(x), _TYPE[x.dtype], b, _pitch(b), b_scale, _pitch(b_scale), (_OUT_DTYPE[out], m, n), n, OUT[out], m, n, k)
+
+
 def mx_to_k_major(src, src_scale, k: int, n: int):
     """codes [batch, k, n] (or [k, n]) with scales [batch, k/64, n, 2] -> K-contiguous codes [batch, n, k], scales [batch, n, k/32]."""
     _need_cuda(src, src_scale)

@@ -145,6 +145,21 @@ int cmx_mx_gemm(const uint8_t* a, uint32_t lda, const uint8_t* a_scale, uint32_t
                 uint32_t n, uint32_t k, int fmt, int out_type, cmx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * A few rows of activations times MXFP4 weights (W4A16; no counterpart in the reference, whose matmuls quantise both
+ * operands):  out[m, n] = x[m, k] . deq(b)[n, k]^T, x as it is.  For a decode step, where reading the weights is the time;
+ * any m is right, but from some 64 rows on quantised activations and cmx_mx_gemm are the faster way.
+ *
+ *   x        [m, k] of x_type (CMX_OUT_BF16 / FP16 / FP32), pitch ld_x elements, elements' alignment
+ *   b        E2M1 codes [n, k/2], even column in the low nibble, pitch ld_b bytes; rows 16-byte aligned
+ *   b_scale  E8M0 [n, >= k/32], pitch ld_bs bytes (as the quantizer writes it for a weight)
+ *   out      [m, n] of out_type, pitch ld_out elements
+ * Products are exact (fp16 and fp32 activations are split into bf16 pieces that add up to them) and sums are fp32.  k a multiple of 32.
+ * ---------------------------------------------------------------------------------------- */
+int cmx_mxfp4_gemv(const void* x, uint32_t ld_x, int x_type, const uint8_t* b, uint32_t ld_b, const uint8_t* b_scale,
+                   uint32_t ld_bs, void* out, uint32_t ld_out, int out_type, uint32_t m, uint32_t n, uint32_t k,
+                   cmx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Grouped MX matmul over ragged expert groups.
  * Replaces the AIC tile loops of Ascend950GmmAllToAllKernel
  * (include/catccos/dgemm/kernel/ascend950_gmm_alltoall.hpp:219-324) and
