@@ -68,6 +68,8 @@ SIGNATURES = {
     "cmx_quant_scatter": (i32, [vp, u32, i32p, u8p, u32, u8p, u32, u32, u32, u32, vp]),
     "cmx_quant_scatter_zeroed": (i32, [vp, u32, i32p, u8p, u32, u8p, u32, u32, u32, u32, vp]),
     "cmx_moe_token_unpermute": (i32, [vp, u32, u32, i32p, f32p, vp, u32, u32, u32, u32, vp]),
+    "cmx_mxfp4_moe_ffn_workspace_bytes": (sz, [u32, u32, u32]),
+    "cmx_mxfp4_moe_ffn": (i32, [vp, i32p, f32p, u8p, u8p, u8p, u8p, vp, u8p, u32, u32, u32, u32, u32, vp]),
     "catccos_ascend950_symmetric_bytes": (u64, []),
     "catccos_ascend950_dispatch_ffn_combine_workspace_bytes": (sz, [u32, u32, u32, u32, u32, i32]),
     "catccos_ascend950_dispatch_ffn_combine": (i32, [u32, vp, u64, u8p, u8p, u8p, u8p, u8p, u8p, u8p, u8p, u8p, u8p,

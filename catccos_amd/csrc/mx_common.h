@@ -49,6 +49,7 @@ int preload_quant_kernels();
 int preload_norm_kernels();
 int preload_gating_kernels();
 int preload_gemv_kernels();
+int preload_moe_ffn_kernels();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }

@@ -1963,6 +1963,7 @@ extern "C" int cmx_init(void) {
     if (int rc = preload_norm_kernels(); rc != CMX_OK) return rc;
     if (int rc = preload_gating_kernels(); rc != CMX_OK) return rc;
     if (int rc = preload_gemv_kernels(); rc != CMX_OK) return rc;
+    if (int rc = preload_moe_ffn_kernels(); rc != CMX_OK) return rc;
     int cus = 0;
     if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
     void* meta = nullptr;

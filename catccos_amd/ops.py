@@ -440,6 +440,33 @@ def moe_token_unpermute(y: torch.Tensor, src2sorted: torch.Tensor, probs: torch.
     return out
 
 
+def mxfp4_moe_ffn_workspace_bytes(m: int, n: int, top_k: int) -> int:
+    return _lib.load().cmx_mxfp4_moe_ffn_workspace_bytes(index(m), index(n), index(top_k))
+
+
+def mxfp4_moe_ffn(x, expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, workspace=None, out=None) -> torch.Tensor:
+    """dispatch_ffn_combine for a few tokens on MXFP4 weights, with x taken as it is: x bf16 [m, k]; expert_idx int32, gate_weight fp32 [m, top_k];
+    w1 u8 [E, n, k/2] (gate rows then up rows) + w1_scale u8 [E, n, scale_cols(k)]; w2 u8 [E, k, n/4] + w2_scale u8 [E, k, scale_cols(n/2)]
+    -> bf16 [m, k].  A route to an expert outside [0, E) adds nothing."""
+    _here(x, expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, workspace, out)
+    (m, k), (e, n), top_k = x.shape, w1.shape[:2], expert_idx.shape[1]
+    assert x.element_size() == 2 and x.dtype != torch.float16 and expert_idx.dtype == torch.int32 and gate_weight.dtype == torch.float32
+    assert expert_idx.shape == gate_weight.shape == (m, top_k)
+    assert w1.shape == (e, n, k // 2) and w1_scale.shape == (e, n, scale_cols(k)) and w2.shape == (e, k, n // 4) and w2_scale.shape == (e, k, scale_cols(n // 2))
+    for t in (x, expert_idx, gate_weight, w1, w1_scale, w2, w2_scale):
+        assert t.is_contiguous()
+    for t in (w1, w1_scale, w2, w2_scale):
+        assert t.dtype == torch.uint8
+    need = mxfp4_moe_ffn_workspace_bytes(m, n, top_k)
+    if workspace is None:
+        workspace = _empty(x, torch.uint8, max(need, 1))
+    if out is None:
+        out = _empty(x, x.dtype, m, k)
+    assert workspace.is_contiguous() and workspace.nbytes >= need and out.shape == x.shape and out.dtype == x.dtype and out.is_contiguous()
+    _launch("cmx_mxfp4_moe_ffn", x, expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, out, workspace, m, k, n, e, top_k)
+    return out
+
+
 def ffn_workspace_bytes(m: int, k: int, n: int, experts: int, top_k: int) -> int:
     return _lib.load().catccos_ascend950_dispatch_ffn_combine_workspace_bytes(m, k, n, experts, top_k, 1)
 

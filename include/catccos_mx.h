@@ -410,6 +410,26 @@ int cmx_moe_token_unpermute(const void* y, uint32_t ld_y, uint32_t rows, const i
                             uint32_t top_k, cmx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * The routed FFN of a few tokens on MXFP4 expert weights, activations in bf16 (W4A16): the FFN below at decode, with
+ * nothing quantised on the way (no counterpart in the reference).
+ *   out[t] = sum over r of gate_weight[t, r] * (silu(x[t] . Wg^T) * (x[t] . Wu^T)) . W2^T,  W of expert expert_idx[t, r]
+ * in fp32 with one rounding, at the end (between the two matmuls values keep 16 bits).
+ *
+ *   x            bf16 [m, k];  out bf16 [m, k]
+ *   expert_idx   int32 [m, top_k], gate_weight fp32 [m, top_k]; a route whose index is outside [0, experts) adds nothing
+ *                (experts of another device); an expert may be named twice
+ *   w1 / scale   E2M1 [experts, n, k/2] / E8M0 [experts, n, RoundUp2(k/32)]: rows [0, n/2) gate, [n/2, n) up
+ *   w2 / scale   E2M1 [experts, k, n/4] / E8M0 [experts, k, RoundUp2(n/64)]
+ *   workspace    256-byte aligned, cmx_mxfp4_moe_ffn_workspace_bytes bytes; contents may be garbage on entry
+ * k a multiple of 32, n of 64, top_k <= 64, weights 16-byte aligned.  Any number of tokens is right; 64 of them share one reading of the
+ * weights, so for a prefill cmx_mx_gmm on quantised rows is the faster way.  Equal calls give equal bits.
+ * ---------------------------------------------------------------------------------------- */
+size_t cmx_mxfp4_moe_ffn_workspace_bytes(uint32_t m, uint32_t n, uint32_t top_k);
+int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const float* gate_weight, const uint8_t* w1,
+                      const uint8_t* w1_scale, const uint8_t* w2, const uint8_t* w2_scale, void* out, uint8_t* workspace,
+                      uint32_t m, uint32_t k, uint32_t n, uint32_t experts, uint32_t top_k, cmx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Full single-device MoE FFN: dispatch -> GMM1 -> SwiGLU -> requant -> GMM2 -> combine.
  * Same argument list as CatccosKernel::catccos_ascend950_dispatch_ffn_combine_wrapper
  * (examples/torch_binding/include/catccos_torch_kernel.h:40-44, body
