@@ -7,14 +7,19 @@
 // others, which become the columns of its matrix instructions.  a is kept as two bf16 halves whose sum carries 16 bits, so that out is
 // rounded once.  The second kernel's workgroups own rows of W2 for all experts, so that a token's sum over its experts never leaves the workgroup; it
 // is taken in an order that depends on the routing alone.
+#include "mx_launch.h"
 #include "mxfp4_rows.h"
 
+#ifndef CMX_UPW
+#define CMX_UPW 2048
+#endif
 namespace cmx {
 namespace {
 
 constexpr uint32_t kTokens = 64;         // of one pass over the weights; more tokens are taken in several
 constexpr uint32_t kMaxTopK = 64;
 constexpr uint32_t kUpWaves = 8, kDownWaves = 8;
+constexpr uint32_t kMaxLds = 150 * 1024; // besides the lists
 
 struct FfnArgs {
     const uint8_t* x;                    // bf16 [m, k]
@@ -27,15 +32,17 @@ struct FfnArgs {
     uint32_t* counts;                    // [m * top_k]: routes of the expert whose first route this is in its pass, 0 elsewhere
     uint16_t* members;                   // [m * top_k, kTokens]: those routes, counted from the pass's first
     uint32_t m, k, half, experts, top_k;
+    uint32_t up_columns, down_columns;   // routes of an expert that one reading of its weights serves
+    uint32_t up_parts;                   // of K: wavefronts of a workgroup that share a row tile of the first matmul
 };
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
-__global__ __launch_bounds__(64 * kUpWaves) void mxfp4_moe_up_kernel(const FfnArgs a) {
-    __shared__ v4f sums[kUpWaves][2][64];
+__global__ __launch_bounds__(64 * kUpWaves, 4) void mxfp4_moe_up_kernel(const FfnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // activations of each wavefront, then sums: [wavefront][gate, up][lane]
     __shared__ uint16_t members[kTokens];
     __shared__ float weights[kTokens];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t token0 = blockIdx.z * kTokens, tokens = min(a.m - token0, kTokens), routes = tokens * a.top_k, first = blockIdx.y;
     if (first >= routes) return;
     const size_t route0 = (size_t)token0 * a.top_k;
@@ -67,47 +74,70 @@ __global__ __launch_bounds__(64 * kUpWaves) void mxfp4_moe_up_kernel(const FfnAr
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x < count) a.members[(route0 + first) * kTokens + threadIdx.x] = members[threadIdx.x];
 
-    const uint32_t blocks = a.k / 32, scale_pitch = (blocks + 1) & ~1u, tile = blockIdx.x * 16;
-    RowsTile<kXBf16, 2, 1, 1> t;                                      // gate rows and their up rows
+    const uint32_t blocks = a.k / 32, scale_pitch = (blocks + 1) & ~1u, part = wave % a.up_parts;
+    const uint32_t tile = (blockIdx.x * (kUpWaves / a.up_parts) + wave / a.up_parts) * 16;
+    const bool works = tile < a.half;                                 // (the last workgroup of an expert may have wavefronts to spare)
+    RowsTile<kXBf16, 2> t;                                            // gate rows and their up rows
     t.blocks = blocks;
-    t.plane = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const size_t row = (size_t)e * (2 * a.half) + i * a.half + tile + (lane & 15);
+        const size_t row = (size_t)e * (2 * a.half) + i * a.half + (works ? tile : 0) + (lane & 15);
         t.a[i] = a.w1 + row * (a.k / 2) + (lane >> 4) * 16;
-        t.scale[i] = a.w1_scale + row * scale_pitch + (lane >> 4);
+        t.scale[i] = a.w1_scale + row * scale_pitch;
     }
-    for (uint32_t c0 = 0; c0 < count; c0 += 16) {
-        const uint32_t c = min(c0 + (lane & 15), count - 1);          // (columns past the last repeat it, and are not stored)
-        t.x[0] = a.x + ((size_t)(token0 + members[c] / a.top_k) * a.k + (lane >> 4) * 32) * 2;
+    XColumns<kXBf16, true> x;
+    x.x = a.x + (size_t)token0 * a.k * 2;
+    x.pitch = (size_t)a.k * 2;
+    x.plane = 0;
+    x.row_bytes = a.k * 2;
+    x.lds = lds + wave * a.up_columns * XTraits<kXBf16>::kPitch;
+    v4f(*const sums)[2][64] = reinterpret_cast<v4f(*)[2][64]>(lds);
+    for (uint32_t c0 = 0; c0 < count; c0 += a.up_columns) {
+        x.columns = min(count - c0, a.up_columns);
+        x.row = members[c0 + min(lane, x.columns - 1)] / a.top_k;
         t.clear();
-        t.run(wave, (blocks + 3) / 4, kUpWaves);
-        if (c0) __syncthreads();
-        sums[wave][0][lane] = t.acc[0][0];
-        sums[wave][1][lane] = t.acc[1][0];
-        __syncthreads();
-        if (threadIdx.x < 256) {
-            const uint32_t l = threadIdx.x >> 2, i = threadIdx.x & 3, col = c0 + (l & 15);
-            float g = 0.0f, u = 0.0f;
+        if (works) t.run(x, part, (blocks + kUnitBlocks - 1) / kUnitBlocks, a.up_parts);
+        if (a.up_parts > 1) {
+            __syncthreads();
+            if (part != 0) {
+                sums[wave][0][lane] = t.acc[0];
+                sums[wave][1][lane] = t.acc[1];
+            }
+            __syncthreads();
+            if (part == 0) {
+                for (uint32_t w = 1; w < a.up_parts; ++w) {
+                    t.acc[0] += sums[wave + w][0][lane];
+                    t.acc[1] += sums[wave + w][1][lane];
+                }
+            }
+            if (c0 + a.up_columns < count) __syncthreads();           // (the next activations go where these sums are)
+        }
+        const uint32_t c = lane & 15;
+        if (part == 0 && works && c < x.columns) {
+            uint32_t lead[2], rest[2];
+            float v[4], w[4];
 #pragma unroll
-            for (uint32_t w = 0; w < kUpWaves; ++w) {
-                g += sums[w][0][l][i];
-                u += sums[w][1][l][i];
+            for (int i = 0; i < 4; ++i) {
+                v[i] = weights[c0 + c] * (silu(t.acc[0][i]) * t.acc[1][i]);
+                const float high = __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
+                w[i] = high == v[i] ? 0.0f : v[i] - high;
             }
-            if (col < count) {
-                const float v = weights[col] * (silu(g) * u), lead = __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
-                const size_t at = ((route0 + members[col]) * a.half + tile + (l >> 4) * 4 + i) * 2;
-                *reinterpret_cast<uint16_t*>(a.act + at) = (uint16_t)(__float_as_uint(v) >> 16);
-                *reinterpret_cast<uint16_t*>(a.act + a.plane + at) = (uint16_t)f32_to_bf16(lead == v ? 0.0f : v - lead);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                lead[i] = __builtin_amdgcn_perm(__float_as_uint(v[2 * i + 1]), __float_as_uint(v[2 * i]), 0x07060302u);
+                rest[i] = cvt_pk_bf16(w[2 * i], w[2 * i + 1]);
             }
+            const size_t at = ((route0 + members[c0 + c]) * a.half + tile + (lane >> 4) * 4) * 2;
+            __builtin_memcpy(a.act + at, lead, 8);
+            __builtin_memcpy(a.act + a.plane + at, rest, 8);
         }
     }
 }
 
-__global__ __launch_bounds__(64 * kDownWaves) void mxfp4_moe_down_kernel(const FfnArgs a) {
-    extern __shared__ float sums[];                                   // [wavefront][token][16 rows]
+__global__ __launch_bounds__(64 * kDownWaves, 4) void mxfp4_moe_down_kernel(const FfnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // activations of each wavefront; sums: [wavefront][token][16 rows]
     __shared__ uint16_t leaders[kTokens * kMaxTopK];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = blockIdx.x * 16;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tile = blockIdx.x * 16;
     const uint32_t token0 = blockIdx.y * kTokens, tokens = min(a.m - token0, kTokens), routes = tokens * a.top_k;
     const size_t route0 = (size_t)token0 * a.top_k;
     uint32_t experts = 0;
@@ -117,15 +147,22 @@ __global__ __launch_bounds__(64 * kDownWaves) void mxfp4_moe_down_kernel(const F
         if (leads && wave == 0) leaders[experts + __popcll(all & ((1ull << lane) - 1))] = (uint16_t)(r0 + lane);
         experts += __popcll(all);
     }
+    const uint32_t staging = a.down_columns * XTraits<kXPlanes>::kPitch;
+    float* const sums = reinterpret_cast<float*>(lds + kDownWaves * staging);
     for (uint32_t i = threadIdx.x; i < kDownWaves * tokens * 16; i += blockDim.x) sums[i] = 0.0f;
     __syncthreads();
 
-    const uint32_t blocks = a.half / 32, scale_pitch = (blocks + 1) & ~1u, units = (blocks + 3) / 4;
+    const uint32_t blocks = a.half / 32, scale_pitch = (blocks + 1) & ~1u, units = (blocks + kUnitBlocks - 1) / kUnitBlocks;
     uint32_t parts = 1;                                               // of an expert's K, where there are fewer experts than wavefronts
     while (experts * parts < kDownWaves && parts < units) parts *= 2;
-    RowsTile<kXPlanes, 1, 1, 1> t;
+    RowsTile<kXPlanes, 1> t;
     t.blocks = blocks;
-    t.plane = a.plane;
+    XColumns<kXPlanes, true> x;
+    x.x = a.act + route0 * a.half * 2;
+    x.pitch = (size_t)a.half * 2;
+    x.plane = a.plane;
+    x.row_bytes = a.half * 2;
+    x.lds = lds + wave * staging;
     float* const mine = sums + (size_t)wave * tokens * 16;
     for (uint32_t item = wave; item < experts * parts; item += kDownWaves) {
         const uint32_t leader = leaders[item / parts], part = item % parts;
@@ -133,15 +170,16 @@ __global__ __launch_bounds__(64 * kDownWaves) void mxfp4_moe_down_kernel(const F
         const uint32_t count = a.counts[route];
         const size_t row = (size_t)a.idx[route] * a.k + tile + (lane & 15);
         t.a[0] = a.w2 + row * (a.half / 2) + (lane >> 4) * 16;
-        t.scale[0] = a.w2_scale + row * scale_pitch + (lane >> 4);
-        for (uint32_t c0 = 0; c0 < count; c0 += 16) {
-            const uint32_t c = c0 + (lane & 15), member = a.members[route * kTokens + min(c, count - 1)];
-            t.x[0] = a.act + ((route0 + member) * a.half + (lane >> 4) * 32) * 2;
+        t.scale[0] = a.w2_scale + row * scale_pitch;
+        for (uint32_t c0 = 0; c0 < count; c0 += a.down_columns) {
+            x.columns = min(count - c0, a.down_columns);
+            const uint32_t c = lane & 15, member = a.members[route * kTokens + c0 + min(c, x.columns - 1)];
+            x.row = member;
             t.clear();
-            t.run(units * part / parts, units * (part + 1) / parts, 1);
-            if (c < count) {                                          // the columns are different tokens
+            t.run(x, units * part / parts, units * (part + 1) / parts, 1);
+            if (c < x.columns) {                                      // the columns are different tokens
                 v4f* const at = reinterpret_cast<v4f*>(mine + (member / a.top_k) * 16 + (lane >> 4) * 4);
-                *at += t.acc[0][0];
+                *at += t.acc[0];
             }
         }
     }
@@ -194,15 +232,28 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
     CMX_REQUIRE(aligned16(w1) && aligned16(w2), "weights must be 16-byte aligned");
     CMX_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "workspace must be 256-byte aligned");
     CMX_REQUIRE(((reinterpret_cast<uintptr_t>(expert_idx) | reinterpret_cast<uintptr_t>(gate_weight)) & 3u) == 0 &&
-                ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 1u) == 0, "pointers must be aligned to their elements");
+                (reinterpret_cast<uintptr_t>(out) & 1u) == 0, "pointers must be aligned to their elements");
+    CMX_REQUIRE(aligned16(x), "x must be 16-byte aligned");
     const FfnLayout l = ffn_layout(m, n, top_k);
-    const FfnArgs a = {static_cast<const uint8_t*>(x), expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, static_cast<uint8_t*>(out), workspace, l.plane,
-                       reinterpret_cast<uint32_t*>(workspace + l.counts), reinterpret_cast<uint16_t*>(workspace + l.members), m, k, n / 2, experts, top_k};
+    FfnArgs a = {static_cast<const uint8_t*>(x), expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, static_cast<uint8_t*>(out), workspace, l.plane,
+                       reinterpret_cast<uint32_t*>(workspace + l.counts), reinterpret_cast<uint16_t*>(workspace + l.members), m, k, n / 2, experts, top_k, 0, 0, 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const uint32_t passes = ceil_div(m, kTokens), tokens = m < kTokens ? m : kTokens;
-    hipLaunchKernelGGL(mxfp4_moe_up_kernel, dim3(n / 32, tokens * top_k, passes), dim3(64 * kUpWaves), 0, s, a);
+    a.up_columns = (uint64_t)tokens * top_k > 2ull * experts ? 16 : 4;
+    a.up_columns = tokens < a.up_columns ? tokens : a.up_columns;
+    a.down_columns = tokens < 4 ? tokens : 4;
+    // K is shared out where the row tiles of all experts alone would leave the card without enough wavefronts
+    const uint64_t tiles = (uint64_t)(tokens * top_k < experts ? tokens * top_k : experts) * (n / 32);
+    const uint32_t units = ceil_div(k, kUnitK);
+    a.up_parts = 1;
+    while (a.up_parts < kUpWaves && a.up_parts * 2 <= units && tiles * a.up_parts < CMX_UPW) a.up_parts *= 2;
+    if (int rc = allow_dynamic_lds<mxfp4_moe_up_kernel, kMaxLds>(); rc != CMX_OK) return rc;
+    if (int rc = allow_dynamic_lds<mxfp4_moe_down_kernel, kMaxLds>(); rc != CMX_OK) return rc;
+    const uint32_t up_each = a.up_columns * XTraits<kXBf16>::kPitch;
+    hipLaunchKernelGGL(mxfp4_moe_up_kernel, dim3(ceil_div(n / 32, kUpWaves / a.up_parts), tokens * top_k, passes), dim3(64 * kUpWaves), kUpWaves * (up_each > 2048 ? up_each : 2048), s, a);
     CMX_LAUNCH_CHECK();
-    hipLaunchKernelGGL(mxfp4_moe_down_kernel, dim3(k / 16, passes), dim3(64 * kDownWaves), kDownWaves * tokens * 16 * 4, s, a);
+    hipLaunchKernelGGL(mxfp4_moe_down_kernel, dim3(k / 16, passes), dim3(64 * kDownWaves),
+                       kDownWaves * (a.down_columns * XTraits<kXPlanes>::kPitch + tokens * 64), s, a);
     CMX_LAUNCH_CHECK();
     return CMX_OK;
 }

@@ -421,7 +421,7 @@ int cmx_moe_token_unpermute(const void* y, uint32_t ld_y, uint32_t rows, const i
  *   w1 / scale   E2M1 [experts, n, k/2] / E8M0 [experts, n, RoundUp2(k/32)]: rows [0, n/2) gate, [n/2, n) up
  *   w2 / scale   E2M1 [experts, k, n/4] / E8M0 [experts, k, RoundUp2(n/64)]
  *   workspace    256-byte aligned, cmx_mxfp4_moe_ffn_workspace_bytes bytes; contents may be garbage on entry
- * k a multiple of 32, n of 64, top_k <= 64, weights 16-byte aligned.  Any number of tokens is right; 64 of them share one reading of the
+ * k a multiple of 32, n of 64, top_k <= 64, x and weights 16-byte aligned.  Any number of tokens is right; 64 of them share one reading of the
  * weights, so for a prefill cmx_mx_gmm on quantised rows is the faster way.  Equal calls give equal bits.
  * ---------------------------------------------------------------------------------------- */
 size_t cmx_mxfp4_moe_ffn_workspace_bytes(uint32_t m, uint32_t n, uint32_t top_k);

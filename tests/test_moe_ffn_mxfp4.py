@@ -21,7 +21,7 @@ WHOLE = dict(x=4096, idx=4096, gate=4096, w1=4096, w1s=4096, w2=4096, w2s=4096, 
     (dict(k=0), "k must"), (dict(k=48), "k must"), (dict(n=0), "n must"), (dict(n=96), "n must"), (dict(experts=0), "experts"), (dict(experts=1 << 31), "experts"),
     (dict(top_k=0), "top_k"), (dict(top_k=65), "top_k"), (dict(m=1 << 30, top_k=2), "too many tokens"), (dict(m=1 << 23), "too many tokens"),
     (dict(w1=4104), "16-byte"), (dict(w2=4104), "16-byte"), (dict(workspace=4224), "256-byte"), (dict(idx=4098), "aligned"), (dict(gate=4097), "aligned"),
-    (dict(x=4097), "aligned"), (dict(out=4097), "aligned")])
+    (dict(x=4104), "16-byte"), (dict(out=4097), "aligned")])
 def test_bad_arguments_are_refused_before_a_launch(change, message):
     lib = _lib.load()
     assert lib.cmx_mxfp4_moe_ffn(*{**WHOLE, **change}.values()) == -1
