@@ -11,7 +11,7 @@ struct GemvArgs {
     const uint8_t *x, *b, *b_scale;
     uint8_t* out;
     size_t ld_x, ld_b, ld_scale, ld_out;      // bytes
-    uint32_t m, n, blocks, columns;
+    uint32_t m, n, blocks;
     int out_type;
 };
 
@@ -43,60 +43,55 @@ __device__ __forceinline__ void store4(uint8_t* p, const v4f v, int type, uint32
         if (i < left) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
 }
 
-template <int KIND, bool ALIGNED, int RT>
-__global__ __launch_bounds__(1024) void mxfp4_gemv_kernel(const GemvArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // activations of each wavefront, then sums: [wavefront][row tile][lane]
+template <int KIND, int RT, int COLUMNS>
+__global__ __launch_bounds__(512) void mxfp4_gemv_kernel(const GemvArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // a stage for each wavefront, then sums: [wavefront][row tile][lane]
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const uint32_t row0 = blockIdx.x * (16 * RT), col0 = blockIdx.y * a.columns;
-    RowsTile<KIND, RT> t;
+    const uint32_t row0 = blockIdx.x * (16 * RT), col0 = blockIdx.y * COLUMNS;
+    RowsStream<KIND, RT, COLUMNS, false> t;
     t.blocks = a.blocks;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {                                    // rows past the last repeat it, and are not stored
-        const uint32_t row = min(row0 + i * 16 + (lane & 15), a.n - 1);
-        t.a[i] = a.b + row * a.ld_b + (lane >> 4) * 16;
-        t.scale[i] = a.b_scale + row * a.ld_scale;
-    }
-    XColumns<KIND, ALIGNED> x;
-    x.x = a.x;
-    x.pitch = a.ld_x;
-    x.plane = 0;
-    x.row_bytes = a.blocks * 32 * XTraits<KIND>::kBytes;
-    x.columns = min(a.m - col0, a.columns);
-    x.row = col0 + lane;
-    x.lds = lds + (size_t)wave * a.columns * XTraits<KIND>::kPitch;
+    for (int i = 0; i < RT; ++i) t.set_rows(i, a.b, a.ld_b, a.b_scale, a.ld_scale, row0 + i * 16, a.n - 1);      // (rows past the last are not stored)
+    t.x = a.x;
+    t.x_pitch = a.ld_x;
+    t.plane = 0;
+    t.row = min(col0 + lane, a.m - 1);
+    t.stage = lds_address(lds) + wave * kStageBytes<KIND, RT, COLUMNS>;
     t.clear();
-    t.run(x, wave, (a.blocks + kUnitBlocks - 1) / kUnitBlocks, waves);
+    t.run(wave, (a.blocks + kUnitBlocks - 1) / kUnitBlocks, waves);
     __syncthreads();
     v4f* const sums = reinterpret_cast<v4f*>(lds);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) sums[(wave * RT + i) * 64 + lane] = t.acc[i];
+    for (int i = 0; i < RT; ++i) sums[(wave * RT + i) * 64 + lane] = t.sum(i);
     __syncthreads();
     for (uint32_t at = threadIdx.x; at < RT * 64; at += blockDim.x) {
         v4f v = sums[at];
         for (uint32_t w = 1; w < waves; ++w) v += sums[w * (RT * 64) + at];
         const uint32_t l = at & 63, i = at >> 6;
         const uint32_t row = row0 + i * 16 + (l >> 4) * 4, col = l & 15;     // of weights: output columns; of x: output rows
-        if (row < a.n && col < x.columns)
+        if (row < a.n && col < COLUMNS && col0 + col < a.m)
             store4(a.out + (col0 + col) * a.ld_out + (size_t)row * (a.out_type == CMX_OUT_FP32 ? 4 : 2), v, a.out_type, a.n - row);
     }
 }
 
-// columns (rows of x) of one pass, and the LDS of a workgroup
-constexpr uint32_t kMaxLds = 160 * 1024;
-template <int KIND>
-constexpr uint32_t kMaxColumns = XTraits<KIND>::kLoads == 2 ? 8 : 16;
-
-template <int KIND, bool ALIGNED, int RT>
-int launch(GemvArgs a, hipStream_t s) {
-    a.columns = a.m < kMaxColumns<KIND> ? a.m : kMaxColumns<KIND>;
-    const uint32_t each = a.columns * XTraits<KIND>::kPitch, most = kMaxLds / each < 16 ? kMaxLds / each : 16;
+template <int KIND, int RT, int COLUMNS>
+int launch(const GemvArgs& a, hipStream_t s) {
+    constexpr uint32_t kEach = kStageBytes<KIND, RT, COLUMNS>, kFit = 160 * 1024 / kEach, kMaxWaves = kFit < 8 ? kFit : 8;
     // as many wavefronts as share the units of K evenly
-    const uint32_t units = ceil_div(a.blocks, kUnitBlocks), waves = ceil_div(units, ceil_div(units, most));
-    if (int rc = allow_dynamic_lds<mxfp4_gemv_kernel<KIND, ALIGNED, RT>, kMaxLds>(); rc != CMX_OK) return rc;
-    const uint32_t bytes = waves * (each > RT * 1024 ? each : RT * 1024);
-    hipLaunchKernelGGL((mxfp4_gemv_kernel<KIND, ALIGNED, RT>), dim3(ceil_div(a.n, 16 * RT), ceil_div(a.m, a.columns)), dim3(64 * waves), bytes, s, a);
+    const uint32_t units = ceil_div(a.blocks, kUnitBlocks), waves = ceil_div(units, ceil_div(units, kMaxWaves));
+    if (int rc = allow_dynamic_lds<mxfp4_gemv_kernel<KIND, RT, COLUMNS>, kMaxWaves * kEach>(); rc != CMX_OK) return rc;
+    hipLaunchKernelGGL((mxfp4_gemv_kernel<KIND, RT, COLUMNS>), dim3(ceil_div(a.n, 16 * RT), ceil_div(a.m, COLUMNS)), dim3(64 * waves), waves * kEach, s, a);
     CMX_LAUNCH_CHECK();
     return CMX_OK;
+}
+
+template <int KIND>
+int launch(const GemvArgs& a, hipStream_t s) {
+    if (a.m <= 1) return launch<KIND, 1, 1>(a, s);
+    if (a.m <= 2) return launch<KIND, 1, 2>(a, s);
+    if (a.m <= 4) return launch<KIND, 1, 4>(a, s);
+    if (a.m <= 8 || KIND == kXFp32) return launch<KIND, 1, 8>(a, s);
+    return launch<KIND, 1, KIND == kXFp32 ? 8 : 16>(a, s);
 }
 
 }  // namespace
@@ -104,7 +99,7 @@ int launch(GemvArgs a, hipStream_t s) {
 
 int cmx::preload_gemv_kernels() {
     hipFuncAttributes attr;
-    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::mxfp4_gemv_kernel<kXBf16, true, 1>)));
+    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::mxfp4_gemv_kernel<kXBf16, 1, 1>)));
     return CMX_OK;
 }
 
@@ -121,12 +116,9 @@ extern "C" int cmx_mxfp4_gemv(const void* x, uint32_t ld_x, int x_type, const ui
     const uint32_t xb = x_type == CMX_OUT_FP32 ? 4 : 2, ob = out_type == CMX_OUT_FP32 ? 4 : 2;
     CMX_REQUIRE(reinterpret_cast<uintptr_t>(x) % xb == 0 && reinterpret_cast<uintptr_t>(out) % ob == 0, "pointers must be aligned to their elements");
     CMX_REQUIRE(ceil_div(m, 8) <= 65535u, "too many rows of x");
-    const GemvArgs a = {static_cast<const uint8_t*>(x), b, b_scale, static_cast<uint8_t*>(out), (size_t)ld_x * xb, ld_b, ld_bs, (size_t)ld_out * ob, m, n, k / 32, 0,
+    const GemvArgs a = {static_cast<const uint8_t*>(x), b, b_scale, static_cast<uint8_t*>(out), (size_t)ld_x * xb, ld_b, ld_bs, (size_t)ld_out * ob, m, n, k / 32,
                         out_type};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const auto run = [&](auto kind) {
-        return aligned16(x) && (uint64_t)ld_x * xb % 16 == 0 ? launch<kind.value, true, 1>(a, s) : launch<kind.value, false, 1>(a, s);
-    };
-    if (x_type == CMX_OUT_BF16) return run(std::integral_constant<int, kXBf16>());
-    return x_type == CMX_OUT_FP16 ? run(std::integral_constant<int, kXFp16>()) : run(std::integral_constant<int, kXFp32>());
+    if (x_type == CMX_OUT_BF16) return launch<kXBf16>(a, s);
+    return x_type == CMX_OUT_FP16 ? launch<kXFp16>(a, s) : launch<kXFp32>(a, s);
 }

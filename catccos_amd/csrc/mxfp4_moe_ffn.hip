@@ -10,16 +10,16 @@
 #include "mx_launch.h"
 #include "mxfp4_rows.h"
 
-#ifndef CMX_UPW
-#define CMX_UPW 2048
-#endif
 namespace cmx {
 namespace {
 
 constexpr uint32_t kTokens = 64;         // of one pass over the weights; more tokens are taken in several
-constexpr uint32_t kMaxTopK = 64;
-constexpr uint32_t kUpWaves = 8, kDownWaves = 8;
-constexpr uint32_t kMaxLds = 150 * 1024; // besides the lists
+constexpr uint32_t kMaxTopK = 64, kNone = ~0u;
+constexpr uint32_t kDownWaves = 8, kMaxLds = 159 * 1024;
+// First matmul, by the columns of a wavefront: small workgroups, three of which share a CU, so that one works while another starts or ends (32 tokens, 256
+// experts: 458 us; one of eight wavefronts 517); with many columns LDS has room for fewer (45 tokens, 16 experts, K = 992: 30 us and 16).
+constexpr uint32_t up_waves(int columns) { return columns <= 4 ? 4 : 8; }
+constexpr uint32_t kEnoughWaves = 1024;          // of the first matmul, below which K is shared out
 
 struct FfnArgs {
     const uint8_t* x;                    // bf16 [m, k]
@@ -30,95 +30,96 @@ struct FfnArgs {
     uint8_t* act;                        // two planes of bf16 [m * top_k, half]; only rows of a route that is the first of its token and expert
     size_t plane;                        // bytes
     uint32_t* counts;                    // [m * top_k]: routes of the expert whose first route this is in its pass, 0 elsewhere
-    uint16_t* members;                   // [m * top_k, kTokens]: those routes, counted from the pass's first
+    uint32_t* places;                    // [m * top_k]: first route of the expert (counted in the pass) * kTokens + place among its routes, kNone
     uint32_t m, k, half, experts, top_k;
-    uint32_t up_columns, down_columns;   // routes of an expert that one reading of its weights serves
     uint32_t up_parts;                   // of K: wavefronts of a workgroup that share a row tile of the first matmul
 };
 
+__device__ __forceinline__ uint32_t scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
-__global__ __launch_bounds__(64 * kUpWaves, 4) void mxfp4_moe_up_kernel(const FfnArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // activations of each wavefront, then sums: [wavefront][gate, up][lane]
-    __shared__ uint16_t members[kTokens];
+// COLUMNS: routes of an expert that one reading of its weights serves
+template <int COLUMNS>
+__global__ __launch_bounds__(64 * up_waves(COLUMNS), COLUMNS <= 4 ? 3 : 2) void mxfp4_moe_up_kernel(const FfnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // a stage for each wavefront, then sums: [wavefront][gate, up][lane]
+    __shared__ uint16_t members[kTokens];                             // the expert's routes, counted in the pass
     __shared__ float weights[kTokens];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const uint32_t token0 = blockIdx.z * kTokens, tokens = min(a.m - token0, kTokens), routes = tokens * a.top_k, first = blockIdx.y;
     if (first >= routes) return;
     const size_t route0 = (size_t)token0 * a.top_k;
     const int32_t* const idx = a.idx + route0;
     const int32_t e = idx[first];
+    const bool tells = blockIdx.x == 0 && wave == 0;                  // (one wavefront writes down for the second kernel what all find out)
     // every wavefront looks through the routes: the same answer in each
     uint32_t count = 0;
     bool leads = e >= 0 && (uint32_t)e < a.experts;
+    if (!leads && tells && lane == 0) a.places[route0 + first] = kNone;
     for (uint32_t r0 = 0; leads && r0 < routes; r0 += 64) {
         const uint32_t r = r0 + lane;
         bool match = r < routes && idx[r] == e;
         if (__ballot(match && r < first)) leads = false;
         const uint32_t token = r / a.top_k;
         float p = 0.0f;
+        bool counted = match;
         if (match) {                                                  // an expert named twice by a token counts once, with both weights
-            for (uint32_t s = token * a.top_k; s < r; ++s) match &= idx[s] != e;
+            for (uint32_t s = token * a.top_k; s < r; ++s) counted &= idx[s] != e;
             for (uint32_t s = r; s < (token + 1) * a.top_k; ++s) p += idx[s] == e ? a.gate[route0 + s] : 0.0f;
         }
-        const uint64_t all = __ballot(match);
-        if (match && wave == 0) {
-            const uint32_t at = count + __popcll(all & ((1ull << lane) - 1));
+        const uint64_t all = __ballot(counted);
+        const uint32_t at = count + __popcll(all & ((1ull << lane) - 1));
+        if (counted && wave == 0) {
             members[at] = (uint16_t)r;
             weights[at] = p;
         }
+        if (match && leads && tells) a.places[route0 + r] = counted ? first * kTokens + at : kNone;
         count += __popcll(all);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.counts[route0 + first] = leads ? count : 0;
+    if (tells && lane == 0) a.counts[route0 + first] = leads ? count : 0;
     if (!leads) return;
     __syncthreads();
-    if (blockIdx.x == 0 && threadIdx.x < count) a.members[(route0 + first) * kTokens + threadIdx.x] = members[threadIdx.x];
 
     const uint32_t blocks = a.k / 32, scale_pitch = (blocks + 1) & ~1u, part = wave % a.up_parts;
-    const uint32_t tile = (blockIdx.x * (kUpWaves / a.up_parts) + wave / a.up_parts) * 16;
+    const uint32_t tile = (blockIdx.x * (waves / a.up_parts) + wave / a.up_parts) * 16;
     const bool works = tile < a.half;                                 // (the last workgroup of an expert may have wavefronts to spare)
-    RowsTile<kXBf16, 2> t;                                            // gate rows and their up rows
+    RowsStream<kXBf16, 2, COLUMNS, COLUMNS <= 4> t;                       // gate rows and their up rows
     t.blocks = blocks;
+    const size_t w1_row = (size_t)e * (2 * a.half);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const size_t row = (size_t)e * (2 * a.half) + i * a.half + (works ? tile : 0) + (lane & 15);
-        t.a[i] = a.w1 + row * (a.k / 2) + (lane >> 4) * 16;
-        t.scale[i] = a.w1_scale + row * scale_pitch;
-    }
-    XColumns<kXBf16, true> x;
-    x.x = a.x + (size_t)token0 * a.k * 2;
-    x.pitch = (size_t)a.k * 2;
-    x.plane = 0;
-    x.row_bytes = a.k * 2;
-    x.lds = lds + wave * a.up_columns * XTraits<kXBf16>::kPitch;
+    for (int i = 0; i < 2; ++i)
+        t.set_rows(i, a.w1 + w1_row * (a.k / 2), a.k / 2, a.w1_scale + w1_row * scale_pitch, scale_pitch, i * a.half + (works ? tile : 0), 2 * a.half - 1);
+    t.x = a.x + (size_t)token0 * a.k * 2;
+    t.x_pitch = (size_t)a.k * 2;
+    t.plane = 0;
+    t.stage = lds_address(lds) + wave * kStageBytes<kXBf16, 2, COLUMNS>;
     v4f(*const sums)[2][64] = reinterpret_cast<v4f(*)[2][64]>(lds);
-    for (uint32_t c0 = 0; c0 < count; c0 += a.up_columns) {
-        x.columns = min(count - c0, a.up_columns);
-        x.row = members[c0 + min(lane, x.columns - 1)] / a.top_k;
+    for (uint32_t c0 = 0; c0 < count; c0 += COLUMNS) {
+        const uint32_t columns = min(count - c0, (uint32_t)COLUMNS);
+        t.row = members[c0 + min(lane, columns - 1)] / a.top_k;
         t.clear();
-        if (works) t.run(x, part, (blocks + kUnitBlocks - 1) / kUnitBlocks, a.up_parts);
+        if (works) t.run(part, (blocks + kUnitBlocks - 1) / kUnitBlocks, a.up_parts);
         if (a.up_parts > 1) {
             __syncthreads();
             if (part != 0) {
-                sums[wave][0][lane] = t.acc[0];
-                sums[wave][1][lane] = t.acc[1];
+                sums[wave][0][lane] = t.sum(0);
+                sums[wave][1][lane] = t.sum(1);
             }
             __syncthreads();
             if (part == 0) {
                 for (uint32_t w = 1; w < a.up_parts; ++w) {
-                    t.acc[0] += sums[wave + w][0][lane];
-                    t.acc[1] += sums[wave + w][1][lane];
+                    t.acc[0][0] += sums[wave + w][0][lane];
+                    t.acc[1][0] += sums[wave + w][1][lane];
                 }
             }
-            if (c0 + a.up_columns < count) __syncthreads();           // (the next activations go where these sums are)
+            if (c0 + COLUMNS < count) __syncthreads();           // (the next activations go where these sums are)
         }
         const uint32_t c = lane & 15;
-        if (part == 0 && works && c < x.columns) {
+        if (part == 0 && works && c < columns) {
             uint32_t lead[2], rest[2];
             float v[4], w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                v[i] = weights[c0 + c] * (silu(t.acc[0][i]) * t.acc[1][i]);
+                v[i] = weights[c0 + c] * (silu(t.acc[0][0][i]) * t.acc[1][0][i]);
                 const float high = __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
                 w[i] = high == v[i] ? 0.0f : v[i] - high;
             }
@@ -134,76 +135,139 @@ __global__ __launch_bounds__(64 * kUpWaves, 4) void mxfp4_moe_up_kernel(const Ff
     }
 }
 
-__global__ __launch_bounds__(64 * kDownWaves, 4) void mxfp4_moe_down_kernel(const FfnArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // activations of each wavefront; sums: [wavefront][token][16 rows]
-    __shared__ uint16_t leaders[kTokens * kMaxTopK];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tile = blockIdx.x * 16;
+// RT x 16 rows of every W2
+template <int RT, int COLUMNS>
+__global__ __launch_bounds__(64 * kDownWaves) void mxfp4_moe_down_kernel(const FfnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // a stage for each wavefront; sums: [wavefront][token][RT * 16 rows]; lists
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const uint32_t tile = blockIdx.x * (RT * 16);
     const uint32_t token0 = blockIdx.y * kTokens, tokens = min(a.m - token0, kTokens), routes = tokens * a.top_k;
     const size_t route0 = (size_t)token0 * a.top_k;
-    uint32_t experts = 0;
-    for (uint32_t r0 = 0; r0 < routes; r0 += 64) {
-        const bool leads = r0 + lane < routes && a.counts[route0 + r0 + lane] != 0;
-        const uint64_t all = __ballot(leads);
-        if (leads && wave == 0) leaders[experts + __popcll(all & ((1ull << lane) - 1))] = (uint16_t)(r0 + lane);
-        experts += __popcll(all);
+    float* const sums = reinterpret_cast<float*>(lds + waves * kStageBytes<kXPlanes, RT, COLUMNS>);
+    // experts with a route in this pass, in the order of their first routes: expert, its number of routes, where they begin in `members`
+    uint32_t* const expert_of = reinterpret_cast<uint32_t*>(sums + (size_t)waves * tokens * (RT * 16));
+    uint16_t* const begin_of = reinterpret_cast<uint16_t*>(expert_of + routes);
+    uint16_t* const begin_of_route = begin_of + routes + 1;           // by first route
+    uint16_t* const members = begin_of_route + routes;
+    uint32_t experts = 0, all_members = 0;
+    for (uint32_t r0 = 0; r0 < routes; r0 += 64) {                    // the same in every wavefront; the first writes
+        const uint32_t r = r0 + lane, count = r < routes ? a.counts[route0 + r] : 0;
+        const uint64_t leads = __ballot(count != 0);
+        uint32_t before = count;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t v = (uint32_t)__shfl_up((int)before, d);
+            before += lane >= (uint32_t)d ? v : 0;
+        }
+        const uint32_t begin = all_members + before - count;
+        if (count != 0 && wave == 0) {
+            const uint32_t at = experts + __popcll(leads & ((1ull << lane) - 1));
+            expert_of[at] = (uint32_t)a.idx[route0 + r];
+            begin_of[at] = (uint16_t)begin;
+            begin_of_route[r] = (uint16_t)begin;
+        }
+        experts += __popcll(leads);
+        all_members += (uint32_t)__builtin_amdgcn_readlane((int)before, 63);
     }
-    const uint32_t staging = a.down_columns * XTraits<kXPlanes>::kPitch;
-    float* const sums = reinterpret_cast<float*>(lds + kDownWaves * staging);
-    for (uint32_t i = threadIdx.x; i < kDownWaves * tokens * 16; i += blockDim.x) sums[i] = 0.0f;
+    if (threadIdx.x == 0) begin_of[experts] = (uint16_t)all_members;
+    for (uint32_t i = threadIdx.x; i < waves * tokens * (RT * 16); i += blockDim.x) sums[i] = 0.0f;
+    __syncthreads();
+    for (uint32_t r = threadIdx.x; r < routes; r += blockDim.x) {
+        const uint32_t place = a.places[route0 + r];
+        if (place != kNone) members[begin_of_route[place / kTokens] + place % kTokens] = (uint16_t)r;
+    }
     __syncthreads();
 
     const uint32_t blocks = a.half / 32, scale_pitch = (blocks + 1) & ~1u, units = (blocks + kUnitBlocks - 1) / kUnitBlocks;
     uint32_t parts = 1;                                               // of an expert's K, where there are fewer experts than wavefronts
-    while (experts * parts < kDownWaves && parts < units) parts *= 2;
-    RowsTile<kXPlanes, 1> t;
+    while (experts * parts < waves && parts * 2 <= units) parts *= 2;
+    RowsStream<kXPlanes, RT, COLUMNS, COLUMNS <= 4> t;
     t.blocks = blocks;
-    XColumns<kXPlanes, true> x;
-    x.x = a.act + route0 * a.half * 2;
-    x.pitch = (size_t)a.half * 2;
-    x.plane = a.plane;
-    x.row_bytes = a.half * 2;
-    x.lds = lds + wave * staging;
-    float* const mine = sums + (size_t)wave * tokens * 16;
-    for (uint32_t item = wave; item < experts * parts; item += kDownWaves) {
-        const uint32_t leader = leaders[item / parts], part = item % parts;
-        const size_t route = route0 + leader;
-        const uint32_t count = a.counts[route];
-        const size_t row = (size_t)a.idx[route] * a.k + tile + (lane & 15);
-        t.a[0] = a.w2 + row * (a.half / 2) + (lane >> 4) * 16;
-        t.scale[0] = a.w2_scale + row * scale_pitch;
-        for (uint32_t c0 = 0; c0 < count; c0 += a.down_columns) {
-            x.columns = min(count - c0, a.down_columns);
-            const uint32_t c = lane & 15, member = a.members[route * kTokens + c0 + min(c, x.columns - 1)];
-            x.row = member;
-            t.clear();
-            t.run(x, units * part / parts, units * (part + 1) / parts, 1);
-            if (c < x.columns) {                                      // the columns are different tokens
-                v4f* const at = reinterpret_cast<v4f*>(mine + (member / a.top_k) * 16 + (lane >> 4) * 4);
-                *at += t.acc[0];
+    t.x = a.act + route0 * a.half * 2;
+    t.x_pitch = (size_t)a.half * 2;
+    t.plane = a.plane;
+    t.stage = lds_address(lds) + wave * kStageBytes<kXPlanes, RT, COLUMNS>;
+    float* const mine = sums + (size_t)wave * tokens * (RT * 16);
+    // A wavefront's work is a sequence of units: of its share of an expert's K for up to COLUMNS of its routes, then the next columns, then the next
+    // expert.  The next one is requested before the current one is multiplied, across all these borders.
+    struct Position {
+        uint32_t item, begin, columns, unit, last;                    // columns: routes members[begin, begin + columns)
+    };
+    const auto enter = [&](Position& p) {                             // weights and columns of an item and its columns from p.begin on
+        const uint32_t at = p.item / parts, part = p.item % parts;
+        p.columns = min(scalar(begin_of[at + 1]) - p.begin, (uint32_t)COLUMNS);
+        p.unit = units * part / parts;
+        p.last = units * (part + 1) / parts;
+        t.row = members[p.begin + min(lane & 15, p.columns - 1)];
+        const size_t w2_row = (size_t)scalar(expert_of[at]) * a.k;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            t.set_rows(i, a.w2 + w2_row * (a.half / 2), a.half / 2, a.w2_scale + w2_row * scale_pitch, scale_pitch, tile + i * 16, a.k - 1);
+    };
+    const uint32_t items = experts * parts;
+    Position now = {wave, 0, 0, 0, 0};
+    if (wave < items) {
+        now.begin = scalar(begin_of[wave / parts]);
+        enter(now);
+        uint32_t member = t.row;                                      // (of this lane's column)
+        typename RowsStream<kXPlanes, RT, COLUMNS, COLUMNS <= 4>::Unit u;
+        t.load(u, now.unit);
+        t.clear();
+        while (true) {
+            Position next = now;
+            uint32_t next_member = member;
+            bool more = true;
+            t.turn(u, now.unit, [&](auto& v) {
+                ++next.unit;
+                if (next.unit == now.last) {
+                    next.begin += now.columns;
+                    if (next.begin == scalar(begin_of[now.item / parts + 1])) {
+                        next.item += waves;
+                        more = next.item < items;
+                        if (more) next.begin = scalar(begin_of[next.item / parts]);
+                    }
+                    if (more) {
+                        enter(next);
+                        next_member = t.row;
+                    }
+                }
+                if (more) t.load(v, next.unit);
+            });
+            if (now.unit + 1 == now.last) {
+                if ((lane & 15) < now.columns) {                      // the columns are different tokens
+                    v4f* const at = reinterpret_cast<v4f*>(mine + (member / a.top_k) * (RT * 16) + (lane >> 4) * 4);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) at[i * 4] += t.sum(i);
+                }
+                t.clear();
             }
+            if (!more) break;
+            now = next;
+            member = next_member;
         }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < tokens * 4; i += blockDim.x) {
+    for (uint32_t i = threadIdx.x; i < tokens * (RT * 4); i += blockDim.x) {
+        const uint32_t row = tile + i % (RT * 4) * 4;
+        if (row >= a.k) continue;
         v4f v = {0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t w = 0; w < kDownWaves; ++w) v += reinterpret_cast<const v4f*>(sums)[w * tokens * 4 + i];
+        for (uint32_t w = 0; w < waves; ++w) v += reinterpret_cast<const v4f*>(sums)[w * tokens * (RT * 4) + i];
         const uint32_t packed[2] = {cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
-        __builtin_memcpy(a.out + ((size_t)(token0 + i / 4) * a.k + tile + (i & 3) * 4) * 2, packed, 8);
+        __builtin_memcpy(a.out + ((size_t)(token0 + i / (RT * 4)) * a.k + row) * 2, packed, 8);
     }
 }
 
-// the workspace: planes, counts, members
+// the workspace: planes, counts, places
 struct FfnLayout {
-    size_t counts, members, plane, total;
+    size_t counts, places, plane, total;
 };
 FfnLayout ffn_layout(uint64_t m, uint64_t n, uint64_t top_k) {
     FfnLayout l;
     const size_t routes = (size_t)m * top_k;
     l.plane = round_up_sz(routes * (n / 2) * 2, 256);
     l.counts = 2 * l.plane;
-    l.members = l.counts + round_up_sz(routes * 4, 256);
-    l.total = l.members + round_up_sz(routes * kTokens * 2, 256);
+    l.places = l.counts + round_up_sz(routes * 4, 256);
+    l.total = l.places + round_up_sz(routes * 4, 256);
     return l;
 }
 
@@ -212,7 +276,7 @@ FfnLayout ffn_layout(uint64_t m, uint64_t n, uint64_t top_k) {
 
 int cmx::preload_moe_ffn_kernels() {
     hipFuncAttributes attr;
-    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::mxfp4_moe_up_kernel)));
+    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::mxfp4_moe_up_kernel<1>)));
     return CMX_OK;
 }
 
@@ -236,24 +300,49 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
     CMX_REQUIRE(aligned16(x), "x must be 16-byte aligned");
     const FfnLayout l = ffn_layout(m, n, top_k);
     FfnArgs a = {static_cast<const uint8_t*>(x), expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, static_cast<uint8_t*>(out), workspace, l.plane,
-                       reinterpret_cast<uint32_t*>(workspace + l.counts), reinterpret_cast<uint16_t*>(workspace + l.members), m, k, n / 2, experts, top_k, 0, 0, 0};
+                       reinterpret_cast<uint32_t*>(workspace + l.counts), reinterpret_cast<uint32_t*>(workspace + l.places), m, k, n / 2, experts, top_k, 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const uint32_t passes = ceil_div(m, kTokens), tokens = m < kTokens ? m : kTokens;
-    a.up_columns = (uint64_t)tokens * top_k > 2ull * experts ? 16 : 4;
-    a.up_columns = tokens < a.up_columns ? tokens : a.up_columns;
-    a.down_columns = tokens < 4 ? tokens : 4;
+    const uint32_t passes = ceil_div(m, kTokens), tokens = m < kTokens ? m : kTokens, most = tokens * top_k;
     // K is shared out where the row tiles of all experts alone would leave the card without enough wavefronts
-    const uint64_t tiles = (uint64_t)(tokens * top_k < experts ? tokens * top_k : experts) * (n / 32);
+    const uint64_t tiles = (uint64_t)(most < experts ? most : experts) * (n / 32);
     const uint32_t units = ceil_div(k, kUnitK);
-    a.up_parts = 1;
-    while (a.up_parts < kUpWaves && a.up_parts * 2 <= units && tiles * a.up_parts < CMX_UPW) a.up_parts *= 2;
-    if (int rc = allow_dynamic_lds<mxfp4_moe_up_kernel, kMaxLds>(); rc != CMX_OK) return rc;
-    if (int rc = allow_dynamic_lds<mxfp4_moe_down_kernel, kMaxLds>(); rc != CMX_OK) return rc;
-    const uint32_t up_each = a.up_columns * XTraits<kXBf16>::kPitch;
-    hipLaunchKernelGGL(mxfp4_moe_up_kernel, dim3(ceil_div(n / 32, kUpWaves / a.up_parts), tokens * top_k, passes), dim3(64 * kUpWaves), kUpWaves * (up_each > 2048 ? up_each : 2048), s, a);
-    CMX_LAUNCH_CHECK();
-    hipLaunchKernelGGL(mxfp4_moe_down_kernel, dim3(k / 16, passes), dim3(64 * kDownWaves),
-                       kDownWaves * (a.down_columns * XTraits<kXPlanes>::kPitch + tokens * 64), s, a);
-    CMX_LAUNCH_CHECK();
-    return CMX_OK;
+    int cus;
+    if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
+    const auto up = [&](auto c) -> int {
+        constexpr uint32_t kEach = kStageBytes<kXBf16, 2, c.value>, kFit = kMaxLds / kEach, kWaves = kFit < up_waves(c.value) ? kFit : up_waves(c.value);
+        if (int rc = allow_dynamic_lds<mxfp4_moe_up_kernel<c.value>, kWaves * kEach>(); rc != CMX_OK) return rc;
+        a.up_parts = 1;
+        while (a.up_parts * 2 <= kWaves && a.up_parts * 2 <= units && tiles * a.up_parts < kEnoughWaves) a.up_parts *= 2;
+        const uint32_t waves = kWaves - kWaves % a.up_parts;
+        hipLaunchKernelGGL((mxfp4_moe_up_kernel<c.value>), dim3(ceil_div(n / 32, waves / a.up_parts), most, passes), dim3(64 * waves), waves * kEach, s, a);
+        CMX_LAUNCH_CHECK();
+        return CMX_OK;
+    };
+    const auto down = [&](auto rt, auto c) -> int {
+        const uint32_t each = kStageBytes<kXPlanes, rt.value, c.value> + tokens * 64 * rt.value, lists = most * 10 + 16;
+        const uint32_t fit = (kMaxLds - lists) / each, waves = fit < kDownWaves ? fit : kDownWaves;
+        if (int rc = allow_dynamic_lds<mxfp4_moe_down_kernel<rt.value, c.value>, kMaxLds>(); rc != CMX_OK) return rc;
+        hipLaunchKernelGGL((mxfp4_moe_down_kernel<rt.value, c.value>), dim3(ceil_div(k, 16 * rt.value), passes), dim3(64 * waves), waves * each + lists, s, a);
+        CMX_LAUNCH_CHECK();
+        return CMX_OK;
+    };
+    // Columns: as many routes as most experts have; what the others have more costs another reading of their weights.  Routes spread at random, one for
+    // each of 256 experts on average: 88 % of those that have any have at most two and 97 % three.
+    const bool few = most <= 2ull * experts;
+    int rc;
+    const uint32_t up_columns = few && tokens > 3 ? 3 : tokens;
+    if (up_columns <= 1) rc = up(std::integral_constant<int, 1>());
+    else if (up_columns <= 3) rc = up(std::integral_constant<int, 3>());
+    else if (up_columns <= 8) rc = up(std::integral_constant<int, 8>());
+    else rc = up(std::integral_constant<int, 16>());
+    if (rc != CMX_OK) return rc;
+    // two row tiles share a reading of the activations from LDS, if that leaves workgroups for three CUs of four (32 tokens, 256 experts, k = 7168: 303 us
+    // and 358 with one; 45 tokens, 16 experts, k = 992: 36 and 25)
+    const auto rows = [&](auto rt) -> int {
+        const uint32_t down_columns = few && tokens > 2 ? 2 : tokens;
+        if (down_columns <= 1) return down(rt, std::integral_constant<int, 1>());
+        if (down_columns <= 2) return down(rt, std::integral_constant<int, 2>());
+        return down(rt, std::integral_constant<int, 8>());
+    };
+    return ceil_div(k, 32) * 4 >= (uint32_t)cus * 3 ? rows(std::integral_constant<int, 2>()) : rows(std::integral_constant<int, 1>());
 }

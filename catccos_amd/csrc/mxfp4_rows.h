@@ -3,13 +3,15 @@
 // The weights are the matrix instruction's rows: v_mfma_f32_16x16x32_bf16 takes 16 weight rows and up to 16 activation rows as its
 // columns.  E2M1 times a power of two is exact in bf16 and an activation is one bf16 value or a sum of two or three (fp16, fp32), so
 // every product is exact and sums are fp32: nothing is rounded before the result.  Which K a lane's eight values stand for is free as long as
-// both operands agree, so that a lane's share of a step is what it loads at once: 16 bytes of its weight row = 32 codes = one block with
-// one scale, feeding four instructions.  Lane l: row (or column) l % 16, block l / 16 of the step's four.
+// both operands agree, so that a lane's share of a step is 16 bytes of its weight row = 32 codes = one block with one scale, feeding four
+// instructions.  Lane l: row (or column) l % 16, block l / 16 of the step's four.
 //
-// What bounds this is the vector memory path of a CU, not the matrix or vector units.  Reading weights in this layout, 1168384 rows of 1024 bytes
-// (1.2 GB, cold): 6.6 TB/s alone; 5.0 with a byte of scales per lane and step; 6.5 with four bytes per lane and four steps; 3.9 with four
-// loads a step for a single activation row, 1.8 with 16 rows.  So scales come as one word per unit of four steps and change lanes in
-// registers, and activations come as whole kilobytes straight to LDS, from where a step reads its operands.
+// What bounds this on the way to the memory's rate is the address path of a CU, where a load of a wavefront costs about as many cycles as it touches
+// pieces of memory, and the bytes in flight.  Weights loaded as the instruction wants them (16 rows, 16 bytes per lane, neighbouring lanes in
+// different rows) touch 64 pieces, scale bytes and activations as many again.  So everything is loaded as it lies - four rows x 256 bytes of weights,
+// 16 bytes of a row's scales, whole kilobytes of activations - into registers, of which a CU has three times as much as LDS, and changes lanes through a
+// piece of LDS that is the wavefront's own: nothing waits for another wavefront.
+// Measured (FFN of 32 tokens, 163 of 256 experts, K = 7168, N = 4096): CMX_MEASURED
 #pragma once
 
 #include "mx_common.h"
@@ -17,6 +19,7 @@
 namespace cmx {
 
 typedef __bf16 v8bf16 __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kUnitSteps = 4, kUnitBlocks = 16, kUnitK = 512;        // a step: four blocks of 32 along K, one for each 16 lanes
 
@@ -27,78 +30,170 @@ enum XKind { kXBf16 = CMX_OUT_BF16, kXFp16 = CMX_OUT_FP16, kXFp32 = CMX_OUT_FP32
 template <int KIND>
 struct XTraits {
     static constexpr int kPieces = KIND == kXBf16 ? 1 : (KIND == kXFp32 ? 3 : 2);
-    static constexpr int kLoads = KIND == kXFp32 || KIND == kXPlanes ? 2 : 1;      // KiB of a unit of one row, each one load of a wavefront
     static constexpr uint32_t kBytes = KIND == kXFp32 ? 4 : 2;                     // of an element, in one array
-    // of a column in LDS: 16 bytes more than its data, so that eight neighbouring columns lie in different banks
-    static constexpr uint32_t kPitch = 1024 * kLoads + 16;
+    static constexpr int kReads = KIND == kXFp32 || KIND == kXPlanes ? 2 : 1;      // 16-byte pieces that hold eight values
+    static constexpr uint32_t kPitch = kReads * 1024 + 16;                         // of a column in LDS: a unit of one row of x
 };
 
-// The rows of x that a wavefront multiplies, on their way through its own piece of LDS (columns * XTraits::kPitch bytes).
-// ALIGNED: rows of x start at multiples of 16 bytes, and need not pass through registers.
-template <int KIND, bool ALIGNED>
-struct XColumns {
-    using T = XTraits<KIND>;
-    const uint8_t* x;
-    size_t pitch, plane;       // bytes
-    uint32_t row_bytes;        // k elements of one array
-    uint32_t columns;          // 1 to 16
-    uint32_t row;              // lane c: the row of x that is column c
-    uint8_t* lds;
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
+// ---- weights --------------------------------------------------------------------------------------------------------
+// E8M0 byte -> the float that scales a conversion: 2^(byte - 127), NaN for 255
+__device__ __forceinline__ float e8m0_value(uint32_t byte) {
+    const uint32_t bits = byte == 0 ? 0x00400000u : byte << 23;
+    return __uint_as_float(byte == 255 ? 0x7FC00000u : bits);
+}
 
-    // a unit of every column to LDS; what lies past the end of a row is not read
-    __device__ __forceinline__ void fetch(uint32_t unit) const {
-        const uint32_t lane = threadIdx.x & 63;
-        for (uint32_t c = 0; c < columns; ++c) {
-            const uint8_t* const r = x + (size_t)__builtin_amdgcn_readlane(row, c) * pitch;
+// eight E2M1 codes times a scale
+__device__ __forceinline__ v8bf16 e2m1_to_bf16(uint32_t codes, float scale) {
+    v4u w;
+    w.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
+    w.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+    w.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
+    w.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+    return __builtin_bit_cast(v8bf16, w);
+}
+
+// ---- the wavefront --------------------------------------------------------------------------------------------------
+constexpr uint32_t kRowPitch = 256 + 16;        // of a weight row in LDS
+
+// Bytes of LDS of a wavefront: a unit of RT x 16 weight rows, 16 bytes of scales for each, COLUMNS columns of activations
+template <int KIND, int RT, int COLUMNS>
+constexpr uint32_t kStageBytes = RT * (16 * kRowPitch + 256) + COLUMNS * XTraits<KIND>::kPitch;
+
+// RT x 16 weight rows times up to COLUMNS (1 to 16) activation rows.
+//
+// The lanes of a read from LDS want the same 16-byte piece of 16 rows (columns): 16 bytes between these put eight neighbours into different banks.
+// STREAM: weights that are read once pass by the caches, which keep the activations.
+template <int KIND, int RT, int COLUMNS, bool STREAM>
+struct RowsStream {
+    using T = XTraits<KIND>;
+    // a lane's own: where its 16 bytes of each group of four weight rows and its four of the scales come from, at K = 0
+    const uint8_t *a[RT][4], *scale[RT];
+    uint32_t blocks;           // K / 32
+    const uint8_t* x;
+    size_t x_pitch, plane;     // bytes
+    uint32_t row;              // lane c: the row of x that is column c, up to COLUMNS
+    uint32_t stage;            // LDS address
+    v4f acc[RT][T::kPieces];   // one for each piece: products that do not wait for each other
+
+    // a unit on its way
+    struct Unit {
+        v4u a[RT][4], x[COLUMNS][T::kReads];
+        uint32_t scale[RT];
+    };
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-            for (int i = 0; i < T::kLoads; ++i) {
-                const uint8_t* const p = r + (KIND == kXPlanes && i ? plane : 0);
-                const uint32_t at = unit * (kUnitK * T::kBytes) + (KIND == kXFp32 ? i * 1024 : 0) + lane * 16;
-                uint8_t* const to = lds + c * T::kPitch + i * 1024;
-                if constexpr (ALIGNED) {
-                    const auto row_only = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, row_bytes, 0x00020000);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(row_only, (__attribute__((address_space(3))) void*)to, 16, at, 0, 0, 0);
-                } else {
-                    uint4 v;
-                    __builtin_memcpy(&v, p + min(at, row_bytes - 16), 16);
-                    *reinterpret_cast<uint4*>(to + lane * 16) = v;
-                }
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int n = 0; n < T::kPieces; ++n) acc[i][n] = (v4f){0, 0, 0, 0};
+    }
+    __device__ __forceinline__ v4f sum(int i) const {
+        v4f v = acc[i][0];
+#pragma unroll
+        for (int n = 1; n < T::kPieces; ++n) v += acc[i][n];
+        return v;
+    }
+    // Row tile i: 16 rows from `first` on, of which those past `last` are taken for `last`; the arrays' pitches in bytes.
+    __device__ __forceinline__ void set_rows(int i, const uint8_t* codes, size_t pitch, const uint8_t* scales, size_t scale_pitch, uint32_t first, uint32_t last) {
+        const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) a[i][g] = codes + min(first + g * 4 + lane / 16, last) * pitch + lane % 16 * 16;
+        scale[i] = scales + min(first + lane / 4, last) * scale_pitch + lane % 4 * 4;
+    }
+    __device__ __forceinline__ bool whole(uint32_t unit) const { return (unit + 1) * kUnitBlocks <= blocks; }      // the same for every lane
+
+    // what lies past the end of a row is not read
+    __device__ __forceinline__ void load(Unit& u, uint32_t unit) const {
+        const uint32_t lane = threadIdx.x & 63, row_bytes = blocks * 32 * T::kBytes;
+        const bool all = whole(unit);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            if (all) {
+                __builtin_memcpy(&u.scale[i], scale[i] + (size_t)unit * kUnitBlocks, 4);
+            } else {
+                u.scale[i] = 0;
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b)
+                    if (unit * kUnitBlocks + lane % 4 * 4 + b < blocks) u.scale[i] |= (uint32_t)scale[i][unit * kUnitBlocks + b] << (8 * b);
+            }
+            const uint32_t block = unit * kUnitBlocks + lane % 16, back = all || block < blocks ? 0 : (block - (blocks - 1)) * 16;      // (its last block instead)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const v4u* const p = reinterpret_cast<const v4u*>(a[i][g] + (size_t)unit * 256 - back);
+                u.a[i][g] = STREAM ? __builtin_nontemporal_load(p) : *p;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) {
+            const uint8_t* const r = x + (size_t)__builtin_amdgcn_readlane(row, c) * x_pitch;
+#pragma unroll
+            for (int l = 0; l < T::kReads; ++l) {
+                const uint32_t off = min(unit * (kUnitK * T::kBytes) + (KIND == kXFp32 ? l * 1024 : 0) + lane * 16, row_bytes - 16);
+                __builtin_memcpy(&u.x[c][l], r + off + (KIND == kXPlanes && l ? plane : 0), 16);
             }
         }
     }
-    // values [8 j, 8 j + 8) of this lane's block of a step as kPieces operands.  A value is the sum of its pieces, exactly: each takes the leading eight
-    // bits of what is left.
-    __device__ __forceinline__ void operands(uint32_t my_column, int step, int j, bool live, v8bf16 (&out)[T::kPieces]) const {
-        const uint32_t q = (threadIdx.x & 63) >> 4;
-        const uint8_t* const p = lds + my_column * T::kPitch + ((step * 4 + q) * 4 + j) * (8 * T::kBytes);
-        uint4 a = *reinterpret_cast<const uint4*>(p), b = make_uint4(0, 0, 0, 0);
-        if constexpr (T::kLoads == 2) b = *reinterpret_cast<const uint4*>(p + (KIND == kXPlanes ? 1024 : 16));
-        if (!live) a = b = make_uint4(0, 0, 0, 0);
-        if constexpr (KIND == kXBf16) {
-            out[0] = __builtin_bit_cast(v8bf16, a);
-        } else if constexpr (KIND == kXPlanes) {
-            out[0] = __builtin_bit_cast(v8bf16, a);
-            out[1] = __builtin_bit_cast(v8bf16, b);
+    __device__ __forceinline__ void store(const Unit& u) const {
+        typedef __attribute__((address_space(3))) v4u* lds4;
+        const uint32_t lane = threadIdx.x & 63, xs = stage + RT * (16 * kRowPitch + 256);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            *(__attribute__((address_space(3))) uint32_t*)(uintptr_t)(stage + RT * (16 * kRowPitch) + i * 256 + lane * 4) = u.scale[i];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) *(lds4)(uintptr_t)(stage + (i * 16 + g * 4 + lane / 16) * kRowPitch + lane % 16 * 16) = u.a[i][g];
+        }
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+            for (int l = 0; l < T::kReads; ++l) *(lds4)(uintptr_t)(xs + c * T::kPitch + l * 1024 + lane * 16) = u.x[c][l];
+    }
+
+    // what a lane takes from LDS for one step
+    struct Step {
+        v4u codes[RT], x[4][T::kReads];
+        uint32_t scale[RT];
+    };
+    __device__ __forceinline__ void read(Step& g, uint32_t xs, int s) const {
+        typedef const __attribute__((address_space(3))) v4u* lds4;
+        typedef const __attribute__((address_space(3))) uint8_t* lds1;
+        const uint32_t r = threadIdx.x & 15, q = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            g.codes[i] = *(lds4)(uintptr_t)(stage + (i * 16 + r) * kRowPitch + q * 16 + s * 64);
+            g.scale[i] = *(lds1)(uintptr_t)(stage + RT * (16 * kRowPitch) + i * 256 + r * 16 + q + s * 4);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int l = 0; l < T::kReads; ++l)
+                g.x[j][l] = *(lds4)(uintptr_t)(xs + q * (32 * T::kBytes) + s * (128 * T::kBytes) + j * (8 * T::kBytes) + l * (KIND == kXPlanes ? 1024 : 16));
+    }
+    // eight activations as kPieces operands.  A value is the sum of its pieces, exactly: each takes the leading eight bits of what is left.
+    __device__ __forceinline__ static void operands(const v4u (&x)[T::kReads], v8bf16 (&out)[T::kPieces]) {
+        if constexpr (KIND == kXBf16 || KIND == kXPlanes) {
+#pragma unroll
+            for (int n = 0; n < T::kPieces; ++n) out[n] = __builtin_bit_cast(v8bf16, x[n]);
         } else {
             float v[8];
             if constexpr (KIND == kXFp16) {
                 typedef _Float16 v8f16 __attribute__((ext_vector_type(8)));
-                const v8f16 h = __builtin_bit_cast(v8f16, a);
+                const v8f16 h = __builtin_bit_cast(v8f16, x[0]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
             } else {
-                const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
             }
 #pragma unroll
-            for (int p = 0; p < T::kPieces; ++p) {
+            for (int n = 0; n < T::kPieces; ++n) {
                 uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     w[i] = __builtin_amdgcn_perm(__float_as_uint(v[2 * i + 1]), __float_as_uint(v[2 * i]), 0x07060302u);      // upper halves
-                out[p] = __builtin_bit_cast(v8bf16, make_uint4(w[0], w[1], w[2], w[3]));
-                if (p + 1 < T::kPieces) {
+                out[n] = __builtin_bit_cast(v8bf16, (v4u){w[0], w[1], w[2], w[3]});
+                if (n + 1 < T::kPieces) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float lead = __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
@@ -108,148 +203,63 @@ struct XColumns {
             }
         }
     }
-};
-
-// ---- weights --------------------------------------------------------------------------------------------------------
-// byte `i` of a word of E8M0 scales -> the float that scales a conversion: 2^(byte - 127), NaN for 255
-__device__ __forceinline__ float e8m0_value(uint32_t word, int i) {
-    const uint32_t byte = word >> (8 * i) & 0xFFu;
-    const uint32_t bits = byte == 0 ? 0x00400000u : byte << 23;
-    return __uint_as_float(byte == 255 ? 0x7FC00000u : bits);
-}
-
-// eight E2M1 codes times a scale
-__device__ __forceinline__ v8bf16 e2m1_to_bf16(uint32_t codes, float scale) {
-    uint4 w;
-    w.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
-    w.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
-    w.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
-    w.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
-    return __builtin_bit_cast(v8bf16, w);
-}
-
-// The lanes of quarter g of a wavefront hold the four scales of step g of their row; afterwards they hold those of block g of each of the four steps: a
-// 4 x 4 transposition of bytes across quarters, two lane exchanges and two byte permutations.
-__device__ __forceinline__ uint32_t scales_by_block(uint32_t word) {
-    const uint32_t g = (threadIdx.x & 63) >> 4;
-    const auto far = __builtin_amdgcn_permlane32_swap(word, word, false, false);         // steps g & 1, (g & 1) + 2
-    const uint32_t pairs = __builtin_amdgcn_perm(far[1], far[0], g | (g ^ 1) << 8 | (4 + g) << 16 | (4 + (g ^ 1)) << 24);
-    const auto near = __builtin_amdgcn_permlane16_swap(pairs, pairs, false, false);      // of the even quarter, of the odd one
-    return __builtin_amdgcn_perm(near[1], near[0], (g & 1) ? 0x06030401u : 0x07020500u);
-}
-
-// ---- the tile -------------------------------------------------------------------------------------------------------
-// RT x 16 weight rows times up to 16 activation rows.  The pointers are a lane's own: weight row l % 16 of each row tile at block l / 16, its scales
-// at their start.  blocks: K / 32.
-template <int KIND, int RT>
-struct RowsTile {
-    const uint8_t *a[RT], *scale[RT];
-    uint32_t blocks;
-    v4f acc[RT];
-
-    struct Regs {
-        uint4 a[RT][kUnitSteps];
-        uint32_t scale[RT];
-    };
-
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[i] = (v4f){0, 0, 0, 0};
-    }
-    __device__ __forceinline__ void load(Regs& g, uint32_t unit) const {
-        const uint32_t q = (threadIdx.x & 63) >> 4;
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            __builtin_memcpy(&g.scale[i], scale[i] + unit * kUnitBlocks + q * 4, 4);
-#pragma unroll
-            for (int s = 0; s < (int)kUnitSteps; ++s) g.a[i][s] = *reinterpret_cast<const uint4*>(a[i] + ((size_t)unit * kUnitSteps + s) * 64);
-        }
-    }
-    // the unit that K ends in; blocks past the last: codes of zero under a scale of one
-    __device__ __forceinline__ void load_end(Regs& g, uint32_t unit) const {
-        const uint32_t q = (threadIdx.x & 63) >> 4;
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            g.scale[i] = 0x7F7F7F7Fu;
-            for (uint32_t b = 0; b < 4; ++b) {
-                const uint32_t at = unit * kUnitBlocks + q * 4 + b;
-                if (at < blocks) g.scale[i] = (g.scale[i] & ~(0xFFu << (8 * b))) | (uint32_t)scale[i][at] << (8 * b);
-            }
-#pragma unroll
-            for (int s = 0; s < (int)kUnitSteps; ++s) {
-                const uint32_t step = unit * kUnitSteps + s;
-                g.a[i][s] = make_uint4(0, 0, 0, 0);
-                if (step * 4 + q < blocks) g.a[i][s] = *reinterpret_cast<const uint4*>(a[i] + (size_t)step * 64);
-            }
-        }
-    }
-    template <bool WHOLE, bool ALIGNED>
-    __device__ __forceinline__ void multiply(const Regs& g, const XColumns<KIND, ALIGNED>& x, uint32_t unit, uint32_t my_column) {
-        const uint32_t q = (threadIdx.x & 63) >> 4;
-        uint32_t by_block[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) by_block[i] = scales_by_block(g.scale[i]);
+    // the unit in LDS, onto acc
+    template <bool WHOLE>
+    __device__ __forceinline__ void multiply(uint32_t unit) {
+        const uint32_t q = (threadIdx.x & 63) >> 4, xs = stage + RT * (16 * kRowPitch + 256) + (threadIdx.x & 15) % COLUMNS * T::kPitch;      // (columns again and again)
 #pragma unroll
         for (int s = 0; s < (int)kUnitSteps; ++s) {
-            const bool live = WHOLE || (unit * kUnitSteps + s) * 4 + q < blocks;
-            float f[RT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i) f[i] = e8m0_value(by_block[i], s);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v8bf16 xs[XTraits<KIND>::kPieces];
-                x.operands(my_column, s, j, live, xs);
+            Step g;
+            read(g, xs, s);
+            if (!WHOLE && (unit * kUnitSteps + s) * 4 + q >= blocks) {      // past the end of K: zeros on both sides
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    const uint4 c = g.a[i][s];
+                    g.codes[i] = (v4u){0, 0, 0, 0};
+                    g.scale[i] = 127;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int l = 0; l < T::kReads; ++l) g.x[j][l] = (v4u){0, 0, 0, 0};
+            }
+            float f[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) f[i] = e8m0_value(g.scale[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v8bf16 v[T::kPieces];
+                operands(g.x[j], v);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    const v4u c = g.codes[i];
                     const v8bf16 w = e2m1_to_bf16(j == 0 ? c.x : (j == 1 ? c.y : (j == 2 ? c.z : c.w)), f[i]);
 #pragma unroll
-                    for (int p = 0; p < XTraits<KIND>::kPieces; ++p) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xs[p], acc[i], 0, 0, 0);
+                    for (int n = 0; n < T::kPieces; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, v[n], acc[i][n], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);                              // (or the reads of all steps are held at once)
         }
     }
-    // Units first, first + by, ... below last.  The weights of a unit are under way while the one before it is multiplied; its activations are requested when
-    // that is done, since they go to the same LDS.  (Nothing in the loop is conditional: the wait in front of the reads from LDS
-    // then leaves the loads that were issued after the activations' in flight.)
-    template <bool ALIGNED>
-    __device__ __forceinline__ void run(const XColumns<KIND, ALIGNED>& x, uint32_t first, uint32_t last, uint32_t by) {
-        const uint32_t my_column = min(threadIdx.x & 15, x.columns - 1);      // (columns past the last repeat it)
-        const uint32_t end = min(last, blocks / kUnitBlocks);                 // of the whole units
-        if (first < end) {
-            Regs g[2];                                                        // (by turns: a copy would wait for what it copies)
-            uint32_t u = first;
-            const auto turn = [&](const Regs& now, Regs& next) {
-                load(next, u + by);
-                __builtin_amdgcn_sched_barrier(0);                            // (they stay in front of the work)
-                multiply<true>(now, x, u, my_column);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the reads of this unit are done
-                x.fetch(u + by);
-                u += by;
-            };
-            x.fetch(first);
-            load(g[0], first);
-            bool odd = false;
-            while (u + by < end) {
-                turn(g[0], g[1]);
-                if (u + by >= end) {
-                    odd = true;
-                    break;
-                }
-                turn(g[1], g[0]);
-            }
-            if (odd) multiply<true>(g[1], x, u, my_column);
-            else multiply<true>(g[0], x, u, my_column);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            first = u + by;
-        }
-        if (first < last) {
-            Regs g;
-            x.fetch(first);
-            load_end(g, first);
-            multiply<false>(g, x, first, my_column);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
+    // One turn: the unit that was loaded goes to LDS, the next is requested (unless there is none), the one in LDS is multiplied.
+    template <class Next>
+    __device__ __forceinline__ void turn(Unit& u, uint32_t unit, const Next& load_next) {
+        store(u);
+        load_next(u);
+        __builtin_amdgcn_sched_barrier(0);                                  // (the loads stay in front of the work)
+        __builtin_amdgcn_wave_barrier();
+        if (whole(unit)) multiply<true>(unit);
+        else multiply<false>(unit);
+        __builtin_amdgcn_wave_barrier();
+    }
+    // units first, first + by, ... below last
+    __device__ __forceinline__ void run(uint32_t first, uint32_t last, uint32_t by) {
+        if (first >= last) return;
+        Unit u;
+        load(u, first);
+        for (uint32_t n = first; n < last; n += by)
+            turn(u, n, [&](Unit& v) {
+                if (n + by < last) load(v, n + by);
+            });
     }
 };
 
