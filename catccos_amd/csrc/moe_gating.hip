@@ -7,20 +7,28 @@
 // Whole numbers come out, so the order must be that of the exact values, not of their roundings:
 //   - without a bias, and with one value for each group, the order of the scores is the order of the logits, which is compared
 //     as it is; scores are computed for the chosen experts alone (softmax, not renormalised: the sum over all in addition);
-//   - otherwise c is compared in fp32, and a row in which two values lie closer than fp32 can tell apart (kSoftmaxLoss, kSigmoidLoss), other
+//   - otherwise c is compared in fp32, and a row in which two values lie closer than fp32 can tell apart (score_loss), other
 //     than by equal logits and biases, is done again in 64 bits by its whole wavefront.
 // Work split: LPR lanes hold a row, so that a wavefront works on 64 / LPR rows at a time; an expert is one key of 64 bits that
 // carries value and index, and a round of the choice is one maximum over the lanes' own best keys.
+#include <type_traits>
+
 #include "mx_common.h"
 
+#ifndef CMX_GT
+#define CMX_GT 2048
+#endif
 namespace cmx {
 namespace {
 
 constexpr uint32_t kWaves = 4, kMaxTopK = 64, kMaxGroups = 64, kMaxExperts = 1024;
 
-// Relative error of an fp32 score.  Softmax: exp of z - max (its rounding alone costs |z - max| * 2^-24, and 64 * 2^-24 is reached where the score
-// is 10^-28), sums of up to 1024 terms (16 in a lane, then pairs), one division: below 2^-17.  Sigmoid: exp, one addition, one division: below 2^-21.
-constexpr float kSoftmaxLoss = 0x1p-17f, kSigmoidLoss = 0x1p-21f, kSumLoss = 0x1p-22f, kTiny = 0x1p-90f;
+// How far an fp32 score as the choice computes it may be off.  Softmax, relative: exp2 of (z - max) * log2(e), whose rounding costs d = |z - max| units of 2^-24,
+// sums of up to 1024 terms (16 in a lane, then pairs), a reciprocal and two products: (d + 26) * 2^-24, below 2^-17 to d = 100; scores beyond d = 38 are off
+// by less than kTiny anyway.  Sigmoid: exp2, one addition, one reciprocal: s (1 - s) |z| + 3 s + 1 / 2 units of 2^-24, below 2^-22 for any z, and
+// (|z| + 5) * 2^-24 of a small s, below 2^-18 of it to |z| = 59.
+constexpr float kSumLoss = 0x1p-22f, kTiny = 0x1p-70f;
+__device__ __forceinline__ float score_loss(float s, bool softmax) { return softmax ? 0x1p-17f * s : fminf(0x1p-22f, 0x1p-18f * s); }
 
 struct GateArgs {
     const uint8_t* logits;
@@ -29,6 +37,7 @@ struct GateArgs {
     int32_t* idx;
     float* weight;
     uint32_t tokens, experts, top_k, groups, members, top_groups, group_best;
+    uint32_t by_members;       // ceil(2^20 / members): expert e is in group e * by_members >> 20 (exact: e and members are at most 1024)
     float scale;
     int type, softmax, renormalize;
     int by_logit;              // the order of the logits is the order of the choice
@@ -65,58 +74,63 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
 }
-// the lanes' other value under one step of a butterfly over 64 lanes: step 0..3 inside rows of 16, 4 and 5 across them
-template <int STEP>
-__device__ __forceinline__ uint32_t partner(uint32_t v) {
-    if constexpr (STEP == 0) return dpp<0xB1>(v);                       // lane ^ 1
-    if constexpr (STEP == 1) return dpp<0x4E>(v);                       // lane ^ 2
-    if constexpr (STEP == 2) return dpp<0x141>(v);                      // mirrored in 8
-    if constexpr (STEP == 3) return dpp<0x140>(v);                      // mirrored in 16
-    return (uint32_t)__shfl_xor((int)v, STEP == 4 ? 16 : 32);
+// Butterflies over the 16 or 64 lanes of a row: DPP inside 16 lanes, lane exchanges across them.  op(a, b) gets a lane's value and another's.
+template <class Op>
+__device__ __forceinline__ uint32_t across(uint32_t v, const Op& op, bool half) {
+    const auto r = half ? __builtin_amdgcn_permlane32_swap(v, v, false, false) : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return op(r[0], r[1]);
 }
-template <int STEP>
-__device__ __forceinline__ double partner(double v) {
-    return __hiloint2double((int)partner<STEP>((uint32_t)__double2hiint(v)), (int)partner<STEP>((uint32_t)__double2loint(v)));
-}
-template <int LPR>
-__device__ __forceinline__ double row_max_key(double v) {
-    v = max_key(v, partner<0>(v));
-    v = max_key(v, partner<1>(v));
-    v = max_key(v, partner<2>(v));
-    v = max_key(v, partner<3>(v));
+template <int LPR, class Op>
+__device__ __forceinline__ uint32_t butterfly(uint32_t v, const Op& op) {
+    v = op(v, dpp<0xB1>(v));                                            // lane ^ 1
+    v = op(v, dpp<0x4E>(v));                                            // lane ^ 2
+    v = op(v, dpp<0x141>(v));                                           // mirrored in 8
+    v = op(v, dpp<0x140>(v));                                           // mirrored in 16
     if constexpr (LPR == 64) {
-        v = max_key(v, partner<4>(v));
-        v = max_key(v, partner<5>(v));
+        v = across(v, op, false);
+        v = across(v, op, true);
     }
     return v;
 }
 template <int LPR>
-__device__ __forceinline__ float row_sum(float v) {
-    v += __uint_as_float(partner<0>(__float_as_uint(v)));
-    v += __uint_as_float(partner<1>(__float_as_uint(v)));
-    v += __uint_as_float(partner<2>(__float_as_uint(v)));
-    v += __uint_as_float(partner<3>(__float_as_uint(v)));
-    if constexpr (LPR == 64) {
-        v += __uint_as_float(partner<4>(__float_as_uint(v)));
-        v += __uint_as_float(partner<5>(__float_as_uint(v)));
-    }
-    return v;
+__device__ __forceinline__ float row_sum(float f) {
+    return __uint_as_float(butterfly<LPR>(__float_as_uint(f), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 // the largest value that is a number, -Inf if there is none
 template <int LPR>
-__device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, __uint_as_float(partner<0>(__float_as_uint(v))));
-    v = fmaxf(v, __uint_as_float(partner<1>(__float_as_uint(v))));
-    v = fmaxf(v, __uint_as_float(partner<2>(__float_as_uint(v))));
-    v = fmaxf(v, __uint_as_float(partner<3>(__float_as_uint(v))));
+__device__ __forceinline__ float row_max(float f) {
+    return __uint_as_float(butterfly<LPR>(__float_as_uint(f), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+template <int LPR>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    return butterfly<LPR>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    return __hiloint2double((int)dpp<CTRL>((uint32_t)__double2hiint(v)), (int)dpp<CTRL>((uint32_t)__double2loint(v)));
+}
+template <int LPR>
+__device__ __forceinline__ double row_max_key(double v) {
+    v = max_key(v, dpp<0xB1>(v));
+    v = max_key(v, dpp<0x4E>(v));
+    v = max_key(v, dpp<0x141>(v));
+    v = max_key(v, dpp<0x140>(v));
     if constexpr (LPR == 64) {
-        v = fmaxf(v, __uint_as_float(partner<4>(__float_as_uint(v))));
-        v = fmaxf(v, __uint_as_float(partner<5>(__float_as_uint(v))));
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t lo = (uint32_t)__double2loint(v), hi = (uint32_t)__double2hiint(v);
+            const auto l = half ? __builtin_amdgcn_permlane32_swap(lo, lo, false, false) : __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+            const auto h = half ? __builtin_amdgcn_permlane32_swap(hi, hi, false, false) : __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+            v = max_key(__hiloint2double((int)h[0], (int)l[0]), __hiloint2double((int)h[1], (int)l[1]));
+        }
     }
     return v;
 }
 
 __device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+// what the choice makes do with (score_loss)
+__device__ __forceinline__ float quick_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
+__device__ __forceinline__ float quick_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + quick_exp(-z)); }
 
 // ---- the choice of one row in 64 bits, by a whole wavefront; `value` holds `experts` doubles of LDS, `group_value` one for each group
 __device__ __forceinline__ bool better(double a, uint32_t i, double b, uint32_t j) {          // NaN behind everything
@@ -124,24 +138,64 @@ __device__ __forceinline__ bool better(double a, uint32_t i, double b, uint32_t 
     return a > b || (a == b && i < j);
 }
 
+// c of expert e in 64 bits; softmax: under the row's largest logit and sum of exponentials
+__device__ __forceinline__ double exact_choice(const GateArgs& a, const uint8_t* row, uint32_t e, double most, double sum) {
+    const double z = logit(a, row, e);
+    const double s = !a.softmax ? 1.0 / (1.0 + exp(-z)) : (z == -INFINITY || sum == 0.0 ? 0.0 : exp(z - most) / sum);
+    return s + (a.bias ? (double)a.bias[e] : 0.0);
+}
+// most and sum of exact_choice, by a whole wavefront
+__device__ __forceinline__ void exact_sum(const GateArgs& a, const uint8_t* row, double& most, double& sum) {
+    const uint32_t lane = threadIdx.x & 63;
+    most = -INFINITY;
+    sum = 0.0;
+    if (!a.softmax) return;
+    for (uint32_t e = lane; e < a.experts; e += 64) most = fmax(most, (double)logit(a, row, e));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most = fmax(most, __shfl_xor(most, d));
+    for (uint32_t e = lane; e < a.experts; e += 64) {
+        const double z = logit(a, row, e);
+        if (z != -INFINITY) sum += exp(z - most);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+}
+// The groups of `doubtful` that belong to the `wanted` best of them, their values compared in 64 bits, by a whole wavefront; `value`: a double of LDS per group.
+__device__ __forceinline__ uint64_t choose_groups_exactly(const GateArgs& a, const uint8_t* row, uint64_t doubtful, uint32_t wanted, double* value) {
+    const uint32_t lane = threadIdx.x & 63;
+    double most, sum;
+    exact_sum(a, row, most, sum);
+    for (uint64_t left = doubtful; left; left &= left - 1) {
+        const uint32_t g = (uint32_t)__builtin_ctzll(left);
+        double first = -INFINITY, second = -INFINITY;                       // (NaN as -Inf here: such a row is promised distinct indices only)
+        for (uint32_t j = lane; j < a.members; j += 64) {
+            const double v = fmax(exact_choice(a, row, g * a.members + j, most, sum), -INFINITY);
+            second = fmax(second, fmin(first, v));
+            first = fmax(first, v);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const double f = __shfl_xor(first, d), s = __shfl_xor(second, d);
+            second = fmax(fmax(second, s), fmin(first, f));
+            first = fmax(first, f);
+        }
+        if (lane == 0) value[g] = a.group_best == 2 && a.members > 1 ? first + second : first;
+    }
+    __builtin_amdgcn_wave_barrier();
+    const bool mine = doubtful >> lane & 1ull;
+    uint32_t rank = 0;
+    for (uint64_t left = doubtful; left; left &= left - 1) {
+        const uint32_t h = (uint32_t)__builtin_ctzll(left);
+        if (mine && h != lane) rank += better(value[h], h, value[lane], lane);
+    }
+    return __ballot(mine && rank < wanted);
+}
+
 __device__ __forceinline__ void choose_exactly(const GateArgs& a, const uint8_t* row, double* value, double* group_value, uint2* picks) {
     const uint32_t lane = threadIdx.x & 63;
-    double most = -INFINITY, sum = 0.0;
-    if (a.softmax) {
-        for (uint32_t e = lane; e < a.experts; e += 64) most = fmax(most, (double)logit(a, row, e));
-        for (int d = 32; d > 0; d >>= 1) most = fmax(most, __shfl_xor(most, d));
-        for (uint32_t e = lane; e < a.experts; e += 64) {
-            const double z = logit(a, row, e);
-            const double v = z == -INFINITY ? 0.0 : exp(z - most);
-            value[e] = v;
-            sum += v;
-        }
-        for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    }
-    for (uint32_t e = lane; e < a.experts; e += 64) {
-        const double s = a.softmax ? (sum == 0.0 ? 0.0 : value[e] / sum) : 1.0 / (1.0 + exp(-(double)logit(a, row, e)));
-        value[e] = s + (a.bias ? (double)a.bias[e] : 0.0);
-    }
+    double most, sum;
+    exact_sum(a, row, most, sum);
+    for (uint32_t e = lane; e < a.experts; e += 64) value[e] = exact_choice(a, row, e, most, sum);
     __builtin_amdgcn_wave_barrier();
     uint64_t kept = ~0ull;
     if (a.groups > 1) {
@@ -193,29 +247,53 @@ __device__ __forceinline__ void choose_exactly(const GateArgs& a, const uint8_t*
     __builtin_amdgcn_wave_barrier();
 }
 
+// LDS of a wavefront, in the order in which it lies: doubles first
+template <int LPR, int SLOTS>
+struct GateLds {
+    static constexpr uint32_t kRows = 64 / LPR, kCapacity = LPR * SLOTS, kList = LPR == 16 ? 32 : 0;      // candidates of a row
+    static constexpr uint32_t kOrdWords = kRows * kCapacity > 2 * kCapacity ? kRows * kCapacity : 2 * kCapacity;
+    uint32_t list, scores, picks, ords, group_ords, losses, bytes;
+    __host__ __device__ GateLds(uint32_t groups, uint32_t top_k) {
+        list = groups * 8;                                              // group values in 64 bits before it
+        scores = list + kRows * kList * 8;
+        picks = scores + kRows * (top_k + 2) * 8;
+        ords = picks + kRows * (top_k + 2) * 8;
+        group_ords = ords + kOrdWords * 4;
+        losses = group_ords + kRows * groups * 4;
+        bytes = (losses + kRows * groups * 4 + 7) & ~7u;
+    }
+};
+
 // LPR lanes per row, SLOTS experts per lane
 template <int LPR, int SLOTS>
 __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs a) {
     constexpr int kRows = 64 / LPR, kCapacity = LPR * SLOTS, kChunk = SLOTS < 4 ? SLOTS : 4;
-    constexpr int kOrdWords = kRows * kCapacity > 2 * kCapacity ? kRows * kCapacity : 2 * kCapacity;
-    __shared__ __attribute__((aligned(8))) uint32_t ords_[kWaves][kOrdWords];
-    __shared__ double group_values_[kWaves][kMaxGroups];
-    __shared__ uint32_t group_ords_[kWaves][kRows][kMaxGroups];
-    __shared__ uint2 picks_[kWaves][kRows][kMaxTopK + 1];               // index, order of its value
+    extern __shared__ __attribute__((aligned(8))) uint8_t shared[];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x % LPR, sub = (threadIdx.x & 63) / LPR;
     const uint32_t token = (blockIdx.x * kWaves + wave) * kRows + sub;
     if ((blockIdx.x * kWaves + wave) * kRows >= a.tokens) return;       // (nothing waits for a wavefront)
     const bool live = token < a.tokens;
     const uint8_t* const row = a.logits + (size_t)(live ? token : a.tokens - 1) * a.ld;     // (a row past the last repeats it)
-    uint32_t* const ords = ords_[wave] + sub * kCapacity;
-    uint2* const picks = picks_[wave][sub];
+    const GateLds<LPR, SLOTS> lds(a.groups, a.top_k);
+    uint8_t* const mine = shared + wave * lds.bytes;
+    uint32_t* const ords = reinterpret_cast<uint32_t*>(mine + lds.ords) + sub * kCapacity;              // orders by expert
+    const auto picks_of = [&](uint32_t row) { return reinterpret_cast<uint2*>(mine + lds.picks) + row * (a.top_k + 2); };
+    uint2* const picks = picks_of(sub);                                                                 // index, order of its value
+    float2* const scores = reinterpret_cast<float2*>(mine + lds.scores) + sub * (a.top_k + 2);          // logit, score
     const auto expert = [&](int s) { return (uint32_t)(s / kChunk * kChunk * LPR + lane * kChunk + s % kChunk); };
+    const auto bias = [&](uint32_t e) { return a.bias ? a.bias[e] : 0.0f; };
+    const auto pick_of = [&](double key) { return make_uint2(min(key_expert(key), a.experts - 1), key_ord(key)); };
+    // the bits of a ballot that are this row's
+    const auto row_bits = [&](uint64_t all) { return LPR == 64 ? all : all >> (sub * LPR) & ((1ull << (LPR & 63)) - 1); };
 
-    float z[SLOTS];
+    float z[SLOTS], b[SLOTS];
 #pragma unroll
     for (int s = 0; s < SLOTS; s += kChunk) {
         const uint32_t e = expert(s);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) b[s + i] = 0.0f;
         if (e + kChunk <= a.experts) {
+            if (a.bias) __builtin_memcpy(&b[s], a.bias + e, 4 * kChunk);
             if (a.type == CMX_OUT_FP32) {
                 __builtin_memcpy(&z[s], row + (size_t)e * 4, 4 * kChunk);
             } else {
@@ -226,7 +304,10 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) z[s + i] = e + i < a.experts ? logit(a, row, e + i) : -INFINITY;
+            for (int i = 0; i < kChunk; ++i) {
+                z[s + i] = e + i < a.experts ? logit(a, row, e + i) : -INFINITY;
+                if (a.bias && e + i < a.experts) b[s + i] = a.bias[e + i];
+            }
         }
     }
 
@@ -235,143 +316,298 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
     if (a.softmax) {
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) poisoned |= !(z[s] < INFINITY);
-        poisoned = (__ballot(poisoned) >> (sub * LPR) & (LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1)) != 0;
+        poisoned = row_bits(__ballot(poisoned)) != 0;
     }
     if (a.softmax && !(a.by_logit && a.renormalize)) {
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) most = fmaxf(most, z[s]);
         most = row_max<LPR>(most);
+        if (most == -INFINITY) most = 0.0f;                             // (a row of -Inf: scores of zero)
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) total += z[s] == -INFINITY ? 0.0f : expf(z[s] - most);
+        for (int s = 0; s < SLOTS; ++s) total += quick_exp(z[s] - most);
         total = row_sum<LPR>(total);
     }
-    // a score of fp32
+    // a score that is given away
     const auto score = [&](float v) {
         if (!a.softmax) return sigmoid(v);
         return v == -INFINITY ? 0.0f : expf(v - most) / total;
     };
     uint32_t o[SLOTS];
+    const float share = 1.0f / total;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const uint32_t e = expert(s);
         float c = z[s];
-        if (!a.by_logit) c = (poisoned ? NAN : score(z[s])) + (a.bias && e < a.experts ? a.bias[e] : 0.0f);
-        o[s] = e < a.experts ? ord(c) : 0u;
+        if (!a.by_logit) {
+            c = a.softmax ? (z[s] == -INFINITY ? 0.0f : quick_exp(z[s] - most) * share) : quick_sigmoid(z[s]);
+            c = (poisoned ? NAN : c) + b[s];
+        }
+        o[s] = expert(s) < a.experts ? ord(c) : 0u;
     }
 
-    bool near = false;                                                  // two values that fp32 cannot tell apart
+    bool near = false;                                                  // the row is to be done in 64 bits
+    uint64_t kept = ~0ull;                                              // groups
     if (a.groups > 1) {
+        uint32_t* const group_ords = reinterpret_cast<uint32_t*>(mine + lds.group_ords) + sub * a.groups;
+        float* const losses = reinterpret_cast<float*>(mine + lds.losses) + sub * a.groups;
+        const float largest = a.softmax ? share : 1.0f;
+        const auto enter = [&](uint32_t g, uint32_t first, uint32_t second) {
+            const bool both = a.group_best == 2 && second;
+            const float p = unord(first), q = both ? unord(second) : 0.0f;
+            group_ords[g] = both ? ord(p + q) : first;
+            // how far the sum may be off: without a bias its own size says how large its scores are, with one the row's largest does
+            losses[g] = 2.0f * score_loss(a.bias ? largest : p + q, a.softmax) + kSumLoss * (fabsf(p) + fabsf(q));
+        };
+        const uint32_t over = a.members / kChunk;                       // lanes that a group lies in
+        if (kChunk == 4 && a.members % 4 == 0 && (over & (over - 1)) == 0 && over <= (uint32_t)LPR) {
+            // the two best of a lane's four, then of 2, 4, ... lanes
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) ords[expert(s)] = o[s];
-        __builtin_amdgcn_wave_barrier();
-        uint32_t* const group_ords = group_ords_[wave][sub];
-        for (uint32_t g = lane; g < a.groups; g += LPR) {
-            uint32_t first = 0, second = 0, j = g % a.members;          // (each lane starts elsewhere: no two read one bank)
-            for (uint32_t n = 0; n < a.members; ++n) {
-                const uint32_t v = ords[g * a.members + j];
-                j = j + 1 == a.members ? 0 : j + 1;
-                second = max(second, min(first, v));
-                first = max(first, v);
+            for (int s = 0; s < SLOTS; s += kChunk) {
+                uint32_t first = 0, second = 0;
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) {
+                    second = max(second, min(first, o[s + i]));
+                    first = max(first, o[s + i]);
+                }
+                const auto join = [&](uint32_t f, uint32_t g) {
+                    second = max(max(second, g), min(first, f));
+                    first = max(first, f);
+                };
+                if (over > 1) join(dpp<0xB1>(first), dpp<0xB1>(second));
+                if (over > 2) join(dpp<0x4E>(first), dpp<0x4E>(second));
+                if (over > 4) join(dpp<0x141>(first), dpp<0x141>(second));
+                if (over > 8) join(dpp<0x140>(first), dpp<0x140>(second));
+                if (LPR == 64 && over > 16) join((uint32_t)__shfl_xor((int)first, 16), (uint32_t)__shfl_xor((int)second, 16));
+                if (LPR == 64 && over > 32) join((uint32_t)__shfl_xor((int)first, 32), (uint32_t)__shfl_xor((int)second, 32));
+                const uint32_t g = expert(s) * a.by_members >> 20;
+                if ((lane & (over - 1)) == 0 && g < a.groups) enter(g, first, second);
             }
-            group_ords[g] = a.group_best == 2 && second ? ord(unord(first) + unord(second)) : first;
+        } else {                                                        // groups of other sizes: a lane for each
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s) ords[expert(s)] = o[s];
+            __builtin_amdgcn_wave_barrier();
+            for (uint32_t g = lane; g < a.groups; g += LPR) {
+                uint32_t first = 0, second = 0, j = g % a.members;      // (each lane starts elsewhere: no two read one bank)
+                for (uint32_t n = 0; n < a.members; ++n) {
+                    const uint32_t v = ords[g * a.members + j];
+                    j = j + 1 == a.members ? 0 : j + 1;
+                    second = max(second, min(first, v));
+                    first = max(first, v);
+                }
+                enter(g, first, second);
+            }
         }
         __builtin_amdgcn_wave_barrier();
-        // how far a sum of two scores (each at most 1) and their biases may be off
-        const float loss = 2.0f * (a.softmax ? kSoftmaxLoss : kSigmoidLoss);
-        for (uint32_t g = lane; g < a.groups; g += LPR) {
-            const uint32_t mine = group_ords[g];
-            const float v = unord(mine);
-            uint32_t rank = 0;
-            for (uint32_t h = 0; h < a.groups; ++h) {
-                const uint32_t other = group_ords[h];
-                const float w = unord(other);
-                rank += other > mine || (other == mine && h < g);
-                near |= !a.by_logit && h != g && !(fabsf(v - w) > 2.0f * loss + 4.0f * kSumLoss * (fabsf(v) + fabsf(w) + 1.0f));
+        kept = 0;
+        uint64_t close_kept = 0, close_dropped = 0;
+        for (uint32_t g0 = 0; g0 < a.groups; g0 += LPR) {
+            const uint32_t g = g0 + lane;
+            bool keep = false;
+            uint64_t close = 0;                                         // groups that fp32 cannot tell from this one
+            if (g < a.groups) {
+                const uint32_t mine = group_ords[g];
+                const float v = unord(mine), loss = losses[g];
+                uint32_t rank = 0;
+                for (uint32_t h = 0; h < a.groups; ++h) {
+                    const uint32_t other = group_ords[h];
+                    rank += other > mine || (other == mine && h < g);
+                    if (!a.by_logit && !(fabsf(v - unord(other)) > loss + losses[h] + kTiny)) close |= 1ull << h;
+                }
+                keep = rank < a.top_groups;
             }
-            if (rank >= a.top_groups)
-                for (uint32_t j = 0; j < a.members; ++j) ords[g * a.members + j] = 0;
+            kept |= row_bits(__ballot(keep)) << g0;
+            close_kept |= keep ? 0 : close;
+            close_dropped |= keep ? close : 0;
         }
-        near &= a.top_groups < a.groups;
-        __builtin_amdgcn_wave_barrier();
+        // groups that are close to one on the other side of the border: their values in 64 bits decide
+        near = (close_kept & kept) != 0 || (close_dropped & ~kept) != 0;
+        if (a.groups <= (uint32_t)LPR) {
+            uint64_t rows = __ballot(near && live);
+            const uint64_t doubtful = rows;
+            near = false;
+            while (rows) {                                              // every lane of the wavefront sees the same bits
+                const uint32_t which = (uint32_t)__builtin_ctzll(rows) / LPR;
+                const uint64_t lanes = LPR == 64 ? ~0ull : ((1ull << (LPR & 63)) - 1) << (which * LPR);
+                rows &= ~lanes;
+                const uint64_t groups = (doubtful & lanes) >> (which * LPR & 63);
+                const uint32_t high = __builtin_amdgcn_readlane((uint32_t)(kept >> 32), which * LPR), low = __builtin_amdgcn_readlane((uint32_t)kept, which * LPR);
+                const uint64_t sure = ((uint64_t)high << 32 | low) & ~groups;
+                const uint32_t t = (blockIdx.x * kWaves + wave) * kRows + which;
+                const uint64_t won = choose_groups_exactly(a, a.logits + (size_t)t * a.ld, groups, a.top_groups - (uint32_t)__popcll(sure), reinterpret_cast<double*>(mine));
+                if (sub == which) kept = sure | won;
+            }
+        }
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) o[s] = ords[expert(s)];
+        for (int s = 0; s < SLOTS; ++s) o[s] = kept >> ((expert(s) * a.by_members >> 20) & 63) & 1ull ? o[s] : 0u;
     }
 
-    double key[SLOTS], best = 0.0;
+    // two more than are asked for, to see how near they come
+    const uint32_t choices = a.top_groups * a.members, rounds = a.by_logit ? a.top_k : min(a.top_k + 2, choices);
+    bool chosen = false;
+    if constexpr (LPR == 16) {
+        // No more than `rounds` lanes hold larger values than the rounds-th of the lanes' largest, so everything that is chosen is at least that; as a rule
+        // little else is.  These candidates go to a list, where each counts the larger ones.
+        if (rounds <= 16) {
+            constexpr uint32_t kList = GateLds<LPR, SLOTS>::kList;
+            double* const list = reinterpret_cast<double*>(mine + lds.list) + sub * kList;
+            uint32_t top = 0;
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-        key[s] = make_key(o[s], expert(s));
-        best = max_key(best, key[s]);
+            for (int s = 0; s < SLOTS; ++s) top = max(top, o[s]);
+            uint32_t larger = 0;
+#define CMX_LARGER(I) larger += dpp<0x120 + I>(top) > top;                                    // the lane I places on, around the row
+            CMX_LARGER(1) CMX_LARGER(2) CMX_LARGER(3) CMX_LARGER(4) CMX_LARGER(5) CMX_LARGER(6) CMX_LARGER(7) CMX_LARGER(8)
+            CMX_LARGER(9) CMX_LARGER(10) CMX_LARGER(11) CMX_LARGER(12) CMX_LARGER(13) CMX_LARGER(14) CMX_LARGER(15)
+#undef CMX_LARGER
+            const uint32_t least = max(1u, ~row_max<LPR>(larger < rounds ? ~top : 0u));       // the smallest of those with fewer than `rounds` above
+            uint32_t count = 0;
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s) count += o[s] >= least;
+            uint32_t at = count;                                        // of this lane and those before it
+            at += dpp<0x111>(at);
+            at += dpp<0x112>(at);
+            at += dpp<0x114>(at);
+            at += dpp<0x118>(at);
+            const uint32_t all = row_max<LPR>(at);
+            if (__ballot(all > kList || all < rounds) == 0) {
+                chosen = true;
+                list[lane] = 0.0;
+                list[lane + 16] = 0.0;
+                __builtin_amdgcn_wave_barrier();
+                at -= count;
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s)
+                    if (o[s] >= least) list[at++] = make_key(o[s], expert(s));
+                __builtin_amdgcn_wave_barrier();
+                const double first = list[lane], second = list[lane + 16];
+                const uint32_t longest = max(max(__builtin_amdgcn_readlane(all, 0), __builtin_amdgcn_readlane(all, 16)),
+                                             max(__builtin_amdgcn_readlane(all, 32), __builtin_amdgcn_readlane(all, 48)));
+                uint32_t place = 0, second_place = 0;
+                for (uint32_t i = 0; i < longest; i += 4) {             // (zeros behind the end)
+#pragma unroll
+                    for (uint32_t n = 0; n < 4; ++n) {
+                        const double k = list[i + n];
+                        place += k > first;
+                        second_place += k > second;
+                    }
+                }
+                if (lane < all && place < rounds) picks[place] = pick_of(first);
+                if (lane + 16 < all && second_place < rounds) picks[second_place] = pick_of(second);
+            }
+        }
     }
-    // one more than is asked for, to see how near it comes
-    const uint32_t choices = a.top_groups * a.members, rounds = a.by_logit ? a.top_k : min(a.top_k + 1, choices);
-    for (uint32_t r = 0; r < rounds; ++r) {
-        const double won = row_max_key<LPR>(best);
-        if (lane == 0) picks[r] = make_uint2(key_expert(won), key_ord(won));
-        best = 0.0;
+    if (!chosen) {
+        double key[SLOTS], best = 0.0;
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
-            key[s] = __double_as_longlong(key[s]) == __double_as_longlong(won) ? 0.0 : key[s];
+            key[s] = make_key(o[s], expert(s));
             best = max_key(best, key[s]);
+        }
+        for (uint32_t r = 0; r < rounds; ++r) {
+            const double won = row_max_key<LPR>(best);
+            if (lane == 0) picks[r] = pick_of(won);
+            best = 0.0;
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s) {
+                key[s] = __double_as_longlong(key[s]) == __double_as_longlong(won) ? 0.0 : key[s];
+                best = max_key(best, key[s]);
+            }
         }
     }
     __builtin_amdgcn_wave_barrier();
-    if (!a.by_logit) {
-        // closer than fp32 can tell: values c of scores s
-        const float loss = a.softmax ? kSoftmaxLoss : kSigmoidLoss;
-        const auto close = [&](float c, float s, float d, float t) { return !(fabsf(c - d) > loss * (s + t) + kSumLoss * (fabsf(c) + fabsf(d)) + kTiny); };
-        const auto bias = [&](uint32_t e) { return a.bias ? a.bias[e] : 0.0f; };
-        // Neighbours in the order: of equal logits and biases the lower index comes first, rightly.  Where the last chosen and the first that is
-        // not are such a pair, any other value beside them may lie further down, so all are looked at.
-        bool tied = false;
-        for (uint32_t r = lane; r + 1 < rounds; r += LPR) {
-            const uint2 p = picks[r], q = picks[r + 1];
-            const float zp = logit(a, row, p.x), zq = logit(a, row, q.x);
-            const bool same = zp == zq && bias(p.x) == bias(q.x);
-            near |= !same && close(unord(p.y), score(zp), unord(q.y), score(zq));
-            tied |= same && r + 1 == a.top_k;
-        }
-        tied = (__ballot(tied) >> (sub * LPR) & (LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1)) != 0;
-        if (tied) {
-            const uint32_t last = picks[a.top_k].x;
-            const float zl = logit(a, row, last), sl = score(zl), bl = bias(last);
-            for (uint32_t e = lane; e < a.experts; e += LPR) {
-                if (a.groups > 1 && ords[e] == 0) continue;
-                const float z = logit(a, row, e), s = score(z), b = bias(e);
-                near |= !(z == zl && b == bl) && close(s + b, s, sl + bl, sl);
-            }
-        }
-        uint64_t rows = __ballot(near && live);
-        while (rows) {                                                  // every lane of the wavefront sees the same bits
-            const uint32_t which = (uint32_t)__builtin_ctzll(rows) / LPR;
-            rows &= LPR == 64 ? 0ull : ~(((1ull << (LPR & 63)) - 1) << (which * LPR));
-            const uint32_t t = (blockIdx.x * kWaves + wave) * kRows + which;
-            choose_exactly(a, a.logits + (size_t)t * a.ld, reinterpret_cast<double*>(ords_[wave]), group_values_[wave], picks_[wave][which]);
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
 
-    // weights: scores of the chosen
+    // logits and scores of the chosen and the one behind them
     if (a.softmax && a.by_logit && a.renormalize) {                     // any common factor is as good as the sum over all
         for (uint32_t r = lane; r < a.top_k; r += LPR) most = fmaxf(most, logit(a, row, picks[r].x));
         most = row_max<LPR>(most);
         total = 1.0f;
     }
-    float mine[kMaxTopK / LPR], sum = 0.0f;
+    const auto fetch_scores = [&] {
+        for (uint32_t r = lane; r < rounds; r += LPR) {
+            const float v = logit(a, row, picks[r].x);
+            scores[r] = make_float2(v, poisoned ? NAN : score(v));
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+    fetch_scores();
+    if (!a.by_logit) {
+        // closer than fp32 can tell: values c of scores s
+        const auto close = [&](float c, float s, float d, float t) {
+            return !(fabsf(c - d) > score_loss(s, a.softmax) + score_loss(t, a.softmax) + kSumLoss * (fabsf(c) + fabsf(d)) + kTiny);
+        };
+        // Neighbours in the order: clear, of equal logits and biases (then the lower index comes first, rightly), or close.  Close ones are put in order
+        // by their values in 64 bits, the first that is not chosen among them.  That is all if the second behind is clear of it; if not, more may lie there.
+        bool mend = false, border = false, tied = false, open = false;
+        for (uint32_t r = lane; r + 1 < rounds; r += LPR) {
+            const float2 p = scores[r], q = scores[r + 1];
+            const bool same = p.x == q.x && bias(picks[r].x) == bias(picks[r + 1].x);
+            const bool unclear = !same && close(unord(picks[r].y), p.y, unord(picks[r + 1].y), q.y);
+            mend |= unclear && r < a.top_k;
+            border |= (same || unclear) && r + 1 == a.top_k;
+            tied |= same && r == a.top_k;
+            open |= unclear && r == a.top_k;
+        }
+        mend = row_bits(__ballot(mend)) != 0;
+        border = row_bits(__ballot(border)) != 0;
+        tied = border && row_bits(__ballot(tied)) != 0;
+        near |= border && row_bits(__ballot(open)) != 0;
+        near |= mend && (tied || a.top_k + 1 > (uint32_t)LPR);
+        if (tied && !mend) {
+            const float zl = scores[a.top_k].x, sl = scores[a.top_k].y, bl = bias(picks[a.top_k].x);
 #pragma unroll
-    for (uint32_t i = 0; i < kMaxTopK / LPR; ++i) {
-        const uint32_t r = lane + i * LPR;
-        mine[i] = 0.0f;
-        if (r < a.top_k) mine[i] = poisoned ? NAN : score(logit(a, row, picks[r].x));
-        sum += mine[i];
+            for (int s = 0; s < SLOTS; ++s) {
+                if (o[s] == 0) continue;
+                const float v = logit(a, row, expert(s));
+                near |= !(v == zl && bias(expert(s)) == bl) && close(unord(o[s]), score(v), sl + bl, sl);
+            }
+        }
+        const uint64_t rows = __ballot(near && live);
+        mend &= row_bits(rows) == 0;
+        const uint64_t mended = __ballot(mend);
+        if (mended) {
+            double sum = 0.0;
+            if (a.softmax && a.bias) {
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s) sum += expert(s) < a.experts ? exp((double)logit(a, row, expert(s)) - (double)most) : 0.0;
+#pragma unroll
+                for (int d = 1; d < LPR; d *= 2) sum += __shfl_xor(sum, d);
+            }
+            const uint32_t entries = min(a.top_k + 1, rounds);
+            double* const values = reinterpret_cast<double*>(scores);
+            const bool takes_part = mend && lane < entries;
+            const uint2 pick = picks[takes_part ? lane : 0];
+            double v = 0.0;
+            if (takes_part) {
+                const double zr = scores[lane].x;
+                v = !a.softmax ? 1.0 / (1.0 + exp(-zr)) : (!a.bias ? zr : zr == -INFINITY ? 0.0 : exp(zr - (double)most) / sum);      // (without a bias the order of the logits)
+                v += (double)bias(pick.x);
+            }
+            __builtin_amdgcn_wave_barrier();
+            if (takes_part) values[lane] = v;
+            __builtin_amdgcn_wave_barrier();
+            uint32_t place = 0;
+            if (takes_part)
+                for (uint32_t r = 0; r < entries; ++r) place += r != lane && better(values[r], picks[r].x, v, pick.x);
+            __builtin_amdgcn_wave_barrier();
+            if (takes_part) picks[place] = pick;
+            __builtin_amdgcn_wave_barrier();
+        }
+        for (uint64_t left = rows; left;) {                             // every lane of the wavefront sees the same bits
+            const uint32_t which = (uint32_t)__builtin_ctzll(left) / LPR;
+            left &= LPR == 64 ? 0ull : ~(((1ull << (LPR & 63)) - 1) << (which * LPR));
+            const uint32_t t = (blockIdx.x * kWaves + wave) * kRows + which;
+            choose_exactly(a, a.logits + (size_t)t * a.ld, reinterpret_cast<double*>(mine + lds.ords), reinterpret_cast<double*>(mine), picks_of(which));
+        }
+        if (rows | mended) fetch_scores();
     }
-    if (a.renormalize) sum = row_sum<LPR>(sum);
-#pragma unroll
-    for (uint32_t i = 0; i < kMaxTopK / LPR; ++i) {
-        const uint32_t r = lane + i * LPR;
-        if (r >= a.top_k || !live) continue;
+
+    float sum = 0.0f;
+    if (a.renormalize) {
+        for (uint32_t r = lane; r < a.top_k; r += LPR) sum += scores[r].y;
+        sum = row_sum<LPR>(sum);
+    }
+    for (uint32_t r = lane; r < a.top_k && live; r += LPR) {
+        const float s = scores[r].y;
         a.idx[(size_t)token * a.top_k + r] = (int32_t)picks[r].x;
-        a.weight[(size_t)token * a.top_k + r] = (!a.renormalize ? mine[i] : sum == 0.0f ? 0.0f : mine[i] / sum) * a.scale;
+        a.weight[(size_t)token * a.top_k + r] = (!a.renormalize ? s : sum == 0.0f ? 0.0f : s / sum) * a.scale;
     }
 }
 
@@ -406,23 +642,26 @@ extern "C" int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, 
     CMX_REQUIRE(reinterpret_cast<uintptr_t>(logits) % bytes == 0 && reinterpret_cast<uintptr_t>(bias) % 4 == 0 &&
                 reinterpret_cast<uintptr_t>(expert_idx) % 4 == 0 && reinterpret_cast<uintptr_t>(gate_weight) % 4 == 0, "pointers must be aligned to their elements");
     const GateArgs a = {static_cast<const uint8_t*>(logits), (size_t)ld_logits * bytes, bias, expert_idx, gate_weight, tokens, experts, top_k, groups,
-                        experts / groups, top_groups, group_best, scale, type, score == CMX_SCORE_SOFTMAX, renormalize != 0,
+                        experts / groups, top_groups, group_best, ceil_div(1u << 20, experts / groups), scale, type, score == CMX_SCORE_SOFTMAX, renormalize != 0,
                         !bias && (groups == 1 || group_best == 1 || experts == groups)};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const auto run = [&](auto kernel, uint32_t rows) {
-        hipLaunchKernelGGL(kernel, dim3(ceil_div(tokens, rows * kWaves)), dim3(64 * kWaves), 0, s, a);
+    const auto run = [&](auto lanes, auto slots) {
+        const GateLds<lanes.value, slots.value> lds(groups, top_k);
+        hipLaunchKernelGGL((moe_gating_kernel<lanes.value, slots.value>), dim3(ceil_div(tokens, 64 / lanes.value * kWaves)), dim3(64 * kWaves),
+                           kWaves * lds.bytes, s, a);
     };
-    if (tokens >= 2048 && experts <= 256) {
-        if (experts <= 16) run(moe_gating_kernel<16, 1>, 4);
-        else if (experts <= 32) run(moe_gating_kernel<16, 2>, 4);
-        else if (experts <= 64) run(moe_gating_kernel<16, 4>, 4);
-        else if (experts <= 128) run(moe_gating_kernel<16, 8>, 4);
-        else run(moe_gating_kernel<16, 16>, 4);
-    } else if (experts <= 64) run(moe_gating_kernel<64, 1>, 1);
-    else if (experts <= 128) run(moe_gating_kernel<64, 2>, 1);
-    else if (experts <= 256) run(moe_gating_kernel<64, 4>, 1);
-    else if (experts <= 512) run(moe_gating_kernel<64, 8>, 1);
-    else run(moe_gating_kernel<64, 16>, 1);
+    using std::integral_constant;
+    const auto by_slots = [&](auto lanes) {
+        const uint32_t slots = ceil_div(experts, lanes.value);
+        if (slots <= 1) run(lanes, integral_constant<int, 1>());
+        else if (slots <= 2) run(lanes, integral_constant<int, 2>());
+        else if (slots <= 4) run(lanes, integral_constant<int, 4>());
+        else if (slots <= 8) run(lanes, integral_constant<int, 8>());
+        else run(lanes, integral_constant<int, 16>());
+    };
+    // 16 lanes to a row do less work, 64 are done sooner (CMX_MEASURED)
+    if (tokens >= CMX_GT && experts <= 256) by_slots(integral_constant<int, 16>());
+    else by_slots(integral_constant<int, 64>());
     CMX_LAUNCH_CHECK();
     return CMX_OK;
 }
