@@ -7,17 +7,18 @@
 // Whole numbers come out, so the order must be that of the exact values, not of their roundings:
 //   - without a bias, and with one value for each group, the order of the scores is the order of the logits, which is compared
 //     as it is; scores are computed for the chosen experts alone (softmax, not renormalised: the sum over all in addition);
-//   - otherwise c is compared in fp32, and a row in which two values lie closer than fp32 can tell apart (score_loss), other
-//     than by equal logits and biases, is done again in 64 bits by its whole wavefront.
+//   - otherwise c is compared in fp32, and values that lie closer than fp32 can tell apart (score_loss), other than by equal logits and biases, are
+//     compared again in 64 bits: the groups next to the border between kept and not, the chosen and the first behind them, and the whole row where
+//     that may not be all.  With N(0, 1) logits and sigmoids one row in two thousand has such a pair.
 // Work split: LPR lanes hold a row, so that a wavefront works on 64 / LPR rows at a time; an expert is one key of 64 bits that
-// carries value and index, and a round of the choice is one maximum over the lanes' own best keys.
+// carries value and index.  With 16 lanes to a row the few experts that can be chosen at all are put in a list and count each other; with 64 a round
+// of the choice is one maximum over the lanes' own best keys.
+// Bound by the vector ALU where there are many rows: about 1300 instructions for four rows of 256 in 8 groups.  32768 such rows take 27 us (their 17 MB
+// would take 3), 8192 rows of fp32 logits without groups 6.2, one row 5.0, of which a launch is 2.5.
 #include <type_traits>
 
-#include "mx_common.h"
+#include "mx_launch.h"
 
-#ifndef CMX_GT
-#define CMX_GT 2048
-#endif
 namespace cmx {
 namespace {
 
@@ -49,14 +50,12 @@ __device__ __forceinline__ float logit(const GateArgs& a, const uint8_t* row, ui
     return a.type == CMX_OUT_BF16 ? bf16_to_f32(bits) : (float)__builtin_bit_cast(_Float16, bits);
 }
 
-// ---- order of floats as whole numbers: 0 is left for experts that cannot be chosen, 1 is any NaN, -Inf and upwards lie above
+// ---- order of floats as whole numbers: 0 is left for experts that cannot be chosen; NaN counts as -Inf
 __device__ __forceinline__ uint32_t ord(float f) {
-    const uint32_t u = __float_as_uint(f + 0.0f);                      // (-0 counts as 0)
-    return f != f ? 1u : ((int)u < 0 ? ~u : u | 0x80000000u);
+    const uint32_t u = __float_as_uint(fmaxf(f, -INFINITY) + 0.0f);    // (-0 counts as 0)
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float unord(uint32_t o) {
-    return o <= 1u ? __uint_as_float(0x7FC00000u) : __uint_as_float((int)o < 0 ? o & 0x7FFFFFFFu : ~o);
-}
+__device__ __forceinline__ float unord(uint32_t o) { return __uint_as_float((int)o < 0 ? o & 0x7FFFFFFFu : ~o); }
 
 // ---- keys: order above, index below (the lower index is the larger key), in the mantissa of a double from [1, 2), whose maximum is one instruction
 __device__ __forceinline__ double make_key(uint32_t o, uint32_t e) {
@@ -133,16 +132,14 @@ __device__ __forceinline__ float quick_exp(float v) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float quick_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + quick_exp(-z)); }
 
 // ---- the choice of one row in 64 bits, by a whole wavefront; `value` holds `experts` doubles of LDS, `group_value` one for each group
-__device__ __forceinline__ bool better(double a, uint32_t i, double b, uint32_t j) {          // NaN behind everything
-    if (a != a || b != b) return a != a ? (b != b && i < j) : true;
-    return a > b || (a == b && i < j);
-}
+__device__ __forceinline__ bool better(double a, uint32_t i, double b, uint32_t j) { return a > b || (a == b && i < j); }
+__device__ __forceinline__ double number(double v) { return fmax(v, -INFINITY); }            // NaN counts as -Inf
 
 // c of expert e in 64 bits; softmax: under the row's largest logit and sum of exponentials
 __device__ __forceinline__ double exact_choice(const GateArgs& a, const uint8_t* row, uint32_t e, double most, double sum) {
     const double z = logit(a, row, e);
     const double s = !a.softmax ? 1.0 / (1.0 + exp(-z)) : (z == -INFINITY || sum == 0.0 ? 0.0 : exp(z - most) / sum);
-    return s + (a.bias ? (double)a.bias[e] : 0.0);
+    return number(s + (a.bias ? (double)a.bias[e] : 0.0));
 }
 // most and sum of exact_choice, by a whole wavefront
 __device__ __forceinline__ void exact_sum(const GateArgs& a, const uint8_t* row, double& most, double& sum) {
@@ -167,9 +164,9 @@ __device__ __forceinline__ uint64_t choose_groups_exactly(const GateArgs& a, con
     exact_sum(a, row, most, sum);
     for (uint64_t left = doubtful; left; left &= left - 1) {
         const uint32_t g = (uint32_t)__builtin_ctzll(left);
-        double first = -INFINITY, second = -INFINITY;                       // (NaN as -Inf here: such a row is promised distinct indices only)
+        double first = -INFINITY, second = -INFINITY;
         for (uint32_t j = lane; j < a.members; j += 64) {
-            const double v = fmax(exact_choice(a, row, g * a.members + j, most, sum), -INFINITY);
+            const double v = exact_choice(a, row, g * a.members + j, most, sum);
             second = fmax(second, fmin(first, v));
             first = fmax(first, v);
         }
@@ -179,7 +176,7 @@ __device__ __forceinline__ uint64_t choose_groups_exactly(const GateArgs& a, con
             second = fmax(fmax(second, s), fmin(first, f));
             first = fmax(first, f);
         }
-        if (lane == 0) value[g] = a.group_best == 2 && a.members > 1 ? first + second : first;
+        if (lane == 0) value[g] = a.group_best == 2 && a.members > 1 ? number(first + second) : first;
     }
     __builtin_amdgcn_wave_barrier();
     const bool mine = doubtful >> lane & 1ull;
@@ -214,7 +211,7 @@ __device__ __forceinline__ void choose_exactly(const GateArgs& a, const uint8_t*
                     two = true;
                 }
             }
-            group_value[lane] = a.group_best == 2 && two ? first + second : first;
+            group_value[lane] = a.group_best == 2 && two ? number(first + second) : first;
         }
         __builtin_amdgcn_wave_barrier();
         uint32_t rank = 0;
@@ -250,16 +247,16 @@ __device__ __forceinline__ void choose_exactly(const GateArgs& a, const uint8_t*
 // LDS of a wavefront, in the order in which it lies: doubles first
 template <int LPR, int SLOTS>
 struct GateLds {
-    static constexpr uint32_t kRows = 64 / LPR, kCapacity = LPR * SLOTS, kList = LPR == 16 ? 32 : 0;      // candidates of a row
+    static constexpr uint32_t kRows = 64 / LPR, kCapacity = LPR * SLOTS, kList = LPR == 16 ? 64 : 0;      // candidates of a row
     static constexpr uint32_t kOrdWords = kRows * kCapacity > 2 * kCapacity ? kRows * kCapacity : 2 * kCapacity;
-    uint32_t list, scores, picks, ords, group_ords, losses, bytes;
+    uint32_t list, scores, picks, ords, group_values, losses, bytes;
     __host__ __device__ GateLds(uint32_t groups, uint32_t top_k) {
         list = groups * 8;                                              // group values in 64 bits before it
         scores = list + kRows * kList * 8;
         picks = scores + kRows * (top_k + 2) * 8;
         ords = picks + kRows * (top_k + 2) * 8;
-        group_ords = ords + kOrdWords * 4;
-        losses = group_ords + kRows * groups * 4;
+        group_values = ords + kOrdWords * 4;
+        losses = group_values + kRows * groups * 4;
         bytes = (losses + kRows * groups * 4 + 7) & ~7u;
     }
 };
@@ -341,19 +338,23 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
             c = a.softmax ? (z[s] == -INFINITY ? 0.0f : quick_exp(z[s] - most) * share) : quick_sigmoid(z[s]);
             c = (poisoned ? NAN : c) + b[s];
         }
-        o[s] = expert(s) < a.experts ? ord(c) : 0u;
+        o[s] = ord(c);
+    }
+    if (a.experts < (uint32_t)kCapacity) {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) o[s] = expert(s) < a.experts ? o[s] : 0u;
     }
 
     bool near = false;                                                  // the row is to be done in 64 bits
     uint64_t kept = ~0ull;                                              // groups
     if (a.groups > 1) {
-        uint32_t* const group_ords = reinterpret_cast<uint32_t*>(mine + lds.group_ords) + sub * a.groups;
+        float* const values = reinterpret_cast<float*>(mine + lds.group_values) + sub * a.groups;
         float* const losses = reinterpret_cast<float*>(mine + lds.losses) + sub * a.groups;
         const float largest = a.softmax ? share : 1.0f;
         const auto enter = [&](uint32_t g, uint32_t first, uint32_t second) {
             const bool both = a.group_best == 2 && second;
             const float p = unord(first), q = both ? unord(second) : 0.0f;
-            group_ords[g] = both ? ord(p + q) : first;
+            values[g] = both ? fmaxf(p + q, -INFINITY) : p;             // (not a NaN)
             // how far the sum may be off: without a bias its own size says how large its scores are, with one the row's largest does
             losses[g] = 2.0f * score_loss(a.bias ? largest : p + q, a.softmax) + kSumLoss * (fabsf(p) + fabsf(q));
         };
@@ -398,28 +399,30 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
         }
         __builtin_amdgcn_wave_barrier();
         kept = 0;
-        uint64_t close_kept = 0, close_dropped = 0;
+        float lowest = INFINITY, highest = -INFINITY;                   // of the kept, by the most that they may be too large; of the others, too small
         for (uint32_t g0 = 0; g0 < a.groups; g0 += LPR) {
             const uint32_t g = g0 + lane;
-            bool keep = false;
-            uint64_t close = 0;                                         // groups that fp32 cannot tell from this one
+            uint32_t rank = ~0u;
             if (g < a.groups) {
-                const uint32_t mine = group_ords[g];
-                const float v = unord(mine), loss = losses[g];
-                uint32_t rank = 0;
+                const float v = values[g];
+                rank = 0;
                 for (uint32_t h = 0; h < a.groups; ++h) {
-                    const uint32_t other = group_ords[h];
-                    rank += other > mine || (other == mine && h < g);
-                    if (!a.by_logit && !(fabsf(v - unord(other)) > loss + losses[h] + kTiny)) close |= 1ull << h;
+                    const float w = values[h];
+                    rank += w > v || (w == v && h < g);
                 }
-                keep = rank < a.top_groups;
+                if (rank < a.top_groups) lowest = fminf(lowest, v - losses[g]);
+                else highest = fmaxf(highest, v + losses[g]);
             }
-            kept |= row_bits(__ballot(keep)) << g0;
-            close_kept |= keep ? 0 : close;
-            close_dropped |= keep ? close : 0;
+            kept |= row_bits(__ballot(rank < a.top_groups)) << g0;
         }
-        // groups that are close to one on the other side of the border: their values in 64 bits decide
-        near = (close_kept & kept) != 0 || (close_dropped & ~kept) != 0;
+        // groups that fp32 cannot tell from one on the other side of the border: their values in 64 bits decide
+        lowest = -row_max<LPR>(-lowest);
+        highest = row_max<LPR>(highest);
+        near = !a.by_logit && a.top_groups < a.groups && !(lowest > highest + kTiny);
+        if (near && a.groups <= (uint32_t)LPR) {
+            near = false;
+            if (lane < a.groups) near = kept >> lane & 1ull ? !(values[lane] - losses[lane] > highest + kTiny) : !(values[lane] + losses[lane] < lowest - kTiny);
+        }
         if (a.groups <= (uint32_t)LPR) {
             uint64_t rows = __ballot(near && live);
             const uint64_t doubtful = rows;
@@ -436,8 +439,17 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
                 if (sub == which) kept = sure | won;
             }
         }
+        if (kChunk == 4 && a.members % 4 == 0) {                        // four neighbours are of one group
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) o[s] = kept >> ((expert(s) * a.by_members >> 20) & 63) & 1ull ? o[s] : 0u;
+            for (int s = 0; s < SLOTS; s += kChunk) {
+                const uint32_t all = kept >> ((expert(s) * a.by_members >> 20) & 63) & 1ull ? ~0u : 0u;
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) o[s + i] &= all;
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s) o[s] = kept >> ((expert(s) * a.by_members >> 20) & 63) & 1ull ? o[s] : 0u;
+        }
     }
 
     // two more than are asked for, to see how near they come
@@ -469,28 +481,29 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
             const uint32_t all = row_max<LPR>(at);
             if (__ballot(all > kList || all < rounds) == 0) {
                 chosen = true;
-                list[lane] = 0.0;
-                list[lane + 16] = 0.0;
+                for (uint32_t i = 0; i < kList; i += 16) list[lane + i] = 0.0;
                 __builtin_amdgcn_wave_barrier();
                 at -= count;
 #pragma unroll
                 for (int s = 0; s < SLOTS; ++s)
                     if (o[s] >= least) list[at++] = make_key(o[s], expert(s));
                 __builtin_amdgcn_wave_barrier();
-                const double first = list[lane], second = list[lane + 16];
                 const uint32_t longest = max(max(__builtin_amdgcn_readlane(all, 0), __builtin_amdgcn_readlane(all, 16)),
                                              max(__builtin_amdgcn_readlane(all, 32), __builtin_amdgcn_readlane(all, 48)));
-                uint32_t place = 0, second_place = 0;
-                for (uint32_t i = 0; i < longest; i += 4) {             // (zeros behind the end)
+                for (uint32_t i0 = 0; i0 < longest; i0 += 32) {
+                    const double first = list[i0 + lane], second = list[i0 + 16 + lane];
+                    uint32_t place = 0, second_place = 0;
+                    for (uint32_t i = 0; i < longest; i += 4) {         // (zeros behind the end)
 #pragma unroll
-                    for (uint32_t n = 0; n < 4; ++n) {
-                        const double k = list[i + n];
-                        place += k > first;
-                        second_place += k > second;
+                        for (uint32_t n = 0; n < 4; ++n) {
+                            const double k = list[i + n];
+                            place += k > first;
+                            second_place += k > second;
+                        }
                     }
+                    if (i0 + lane < all && place < rounds) picks[place] = pick_of(first);
+                    if (i0 + 16 + lane < all && second_place < rounds) picks[second_place] = pick_of(second);
                 }
-                if (lane < all && place < rounds) picks[place] = pick_of(first);
-                if (lane + 16 < all && second_place < rounds) picks[second_place] = pick_of(second);
             }
         }
     }
@@ -578,7 +591,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
             if (takes_part) {
                 const double zr = scores[lane].x;
                 v = !a.softmax ? 1.0 / (1.0 + exp(-zr)) : (!a.bias ? zr : zr == -INFINITY ? 0.0 : exp(zr - (double)most) / sum);      // (without a bias the order of the logits)
-                v += (double)bias(pick.x);
+                v = number(v + (double)bias(pick.x));
             }
             __builtin_amdgcn_wave_barrier();
             if (takes_part) values[lane] = v;
@@ -659,8 +672,11 @@ extern "C" int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, 
         else if (slots <= 8) run(lanes, integral_constant<int, 8>());
         else run(lanes, integral_constant<int, 16>());
     };
-    // 16 lanes to a row do less work, 64 are done sooner (CMX_MEASURED)
-    if (tokens >= CMX_GT && experts <= 256) by_slots(integral_constant<int, 16>());
+    // 16 lanes to a row do less work, 64 are done sooner.  Measured in a graph, 64 and 16 lanes, softmax top-8 of 256 / sigmoid in 8 groups: 1024 rows 5.3 and
+    // 6.0 / 7.0 and 9.9 us, 3072 rows 6.3 and 6.1 / 8.7 and 10.1, 4096 rows 7.1 and 6.2 / 10.9 and 10.0, on 256 CUs.
+    int cus;
+    if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
+    if (tokens >= 14u * (uint32_t)cus && experts <= 256) by_slots(integral_constant<int, 16>());
     else by_slots(integral_constant<int, 64>());
     CMX_LAUNCH_CHECK();
     return CMX_OK;

@@ -99,23 +99,25 @@ def _here(*ts):
     for t in ts:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"expected a tensor, not {type(t).__name__}")
-        at = t.get_device()
-        if at < 0:
-            raise ValueError("expected a GPU tensor")
-        if device is None:
-            device = _device()
+        try:
+            at = t.get_device()
+        except AttributeError:
+            raise TypeError(f"expected a tensor, not {type(t).__name__}") from None
         if at != device:
-            raise ValueError(f"expected tensors on the current device ({device}), not on device {at}")
+            if at < 0:
+                raise ValueError("expected a GPU tensor")
+            if device is not None or at != _device():
+                raise ValueError(f"expected tensors on the current device ({_device()}), not on device {at}")
+            device = at
 
 
-def _pitch(t) -> int:
-    """Elements from row to row of a 2-D tensor whose rows lie in one piece (what torch gives a single row as its stride says nothing)."""
-    rows, cols = t.shape
+def _pitch(t, cols: int) -> int:
+    """Elements from row to row of a 2-D tensor of `cols` columns whose rows lie in one piece (the stride of a single row says nothing)."""
+    if t.is_contiguous():
+        return cols
     pitch, step = t.stride()
     assert step == 1 or cols <= 1, "rows must lie in one piece"
-    return pitch if rows > 1 else cols
+    return pitch if t.size(0) > 1 else cols
 
 
 def _bits(value) -> int:
@@ -152,46 +154,45 @@ def mx_dequant(codes: torch.Tensor, scales: torch.Tensor, cols: int, fmt: str = 
     return out
 
 
-def _norm(x, weight, eps, residual, total, y, codes, scales, code_cols, fmt):
-    """cmx_rms_norm_quant; y, codes and scales: a new tensor's dtype and sizes, or None.  Returns the new tensors and the total."""
+def _norm(x, weight, eps, residual, total, y, codes, scales, code_cols, scale_cols, fmt):
+    """cmx_rms_norm_quant; y, codes and scales: a new tensor's dtype and sizes, or None.  Returns the new tensors, the total first among them if it is
+    not the caller's."""
     _here(x, weight, residual, total)
     rows, cols = x.shape
-    assert weight.shape == (cols,) and weight.is_contiguous() and (weight.dtype == x.dtype or weight.dtype == torch.float32)
+    dtype = x.dtype
+    assert weight.shape == (cols,) and weight.is_contiguous() and (weight.dtype == dtype or weight.dtype == torch.float32)
     r_pitch = t_pitch = cols
-    into = total
     if residual is None:
         assert total is None, "a total needs a residual"
     else:
-        assert residual.shape == x.shape and residual.dtype == x.dtype
-        r_pitch = _pitch(residual)
+        assert residual.shape == x.shape and residual.dtype == dtype
+        r_pitch = _pitch(residual, cols)
         if total is None:
-            into = (x.dtype, rows, cols)
+            total = (dtype, rows, cols)
         else:
-            assert total.shape == x.shape and total.dtype == x.dtype
-            t_pitch = _pitch(total)
-    made = _launch("cmx_rms_norm_quant", x, _pitch(x), residual, r_pitch, weight, into, t_pitch, y, cols, codes, code_cols, scales,
-                   0 if scales is None else scales[2], rows, cols, _bits(eps), _TYPE[x.dtype], _TYPE[weight.dtype], FMT[fmt])
-    made = list(made) if made.__class__ is tuple else [made]
-    return made, made.pop(0) if into is not total else total
+            assert total.shape == x.shape and total.dtype == dtype
+            t_pitch = _pitch(total, cols)
+    return _launch("cmx_rms_norm_quant", x, _pitch(x, cols), residual, r_pitch, weight, total, t_pitch, y, cols, codes, code_cols, scales, scale_cols, rows,
+                   cols, _bits(eps), _TYPE[dtype], _TYPE[weight.dtype], FMT[fmt])
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual=None, total=None):
     """x [rows, cols] bf16 / fp16 / fp32, weight [cols] of x's type or fp32 -> (y, t): t = x + residual and y = t / rms(t) * weight, computed in fp32
     and rounded once to x's type.  t is None without a residual; with one it is a new tensor, or `total`, which may be x or the residual."""
-    rows, cols = x.shape
-    (y,), total = _norm(x, weight, eps, residual, total, (x.dtype, rows, cols), None, None, 0, "E4M3")
-    return y, total
+    made = _norm(x, weight, eps, residual, total, (x.dtype, *x.shape), None, None, 0, 0, "E4M3")
+    return (made, total) if made.__class__ is not tuple else (made[1], made[0])
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual=None, fmt: str = "E4M3", want_y: bool = False, total=None):
     """rms_norm straight to MX codes, E4M3, E5M2 or E2M1 to nearest-even: (codes, scales, y|None, t|None), codes and scales as mx_quant gives them but
     made of y before it is rounded."""
     rows, cols = x.shape
-    code_cols = (cols + 1) // 2 if fmt in _FP4 else cols
-    made, total = _norm(x, weight, eps, residual, total, (x.dtype, rows, cols) if want_y else None, (torch.uint8, rows, code_cols),
-                        (torch.uint8, rows, scale_cols(cols)), code_cols, fmt)
-    codes, scales = made[-2:]
-    return codes, scales, made[0] if want_y else None, total
+    code_cols, s_cols = (cols + 1) // 2 if fmt in _FP4 else cols, scale_cols(cols)
+    made = _norm(x, weight, eps, residual, total, (x.dtype, rows, cols) if want_y else None, (torch.uint8, rows, code_cols), (torch.uint8, rows, s_cols),
+                 code_cols, s_cols, fmt)
+    if residual is not None and total is None:
+        total, *made = made
+    return made[-2], made[-1], made[0] if want_y else None, total
 
 
 def mx_gemm(a, a_scale, b, b_scale, k: int, fmt: str = "E4M3", out: str = "bf16") -> torch.Tensor:
@@ -207,7 +208,8 @@ def mxfp4_gemv(x: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: str
     _here(x, b, b_scale)
     (m, k), n = x.shape, b.shape[0]
     assert b.dtype == b_scale.dtype == torch.uint8 and 2 * b.shape[1] == k and b_scale.shape[0] == n and 32 * b_scale.shape[1] >= k
-    return _launch("cmx_mxfp4_gemv", x, _pitch(x), _TYPE[x.dtype], b, _pitch(b), b_scale, _pitch(b_scale), (_OUT_DTYPE[out], m, n), n, OUT[out], m, n, k)
+    return _launch("cmx_mxfp4_gemv", x, _pitch(x, k), _TYPE[x.dtype], b, _pitch(b, b.shape[1]), b_scale, _pitch(b_scale, b_scale.shape[1]),
+                   (_OUT_DTYPE[out], m, n), n, OUT[out], m, n, k)
 
 
 def mx_to_k_major(src, src_scale, k: int, n: int):
@@ -392,7 +394,7 @@ def moe_gating(logits: torch.Tensor, top_k: int, score: str = "softmax", bias=No
     _here(logits, bias)
     tokens, experts = logits.shape
     assert bias is None or (bias.shape == (experts,) and bias.dtype == torch.float32 and bias.is_contiguous())
-    return _launch("cmx_moe_gating", logits, _pitch(logits), _TYPE[logits.dtype], bias, tokens, experts, top_k, SCORE[score], groups, top_groups, group_best,
+    return _launch("cmx_moe_gating", logits, _pitch(logits, experts), _TYPE[logits.dtype], bias, tokens, experts, top_k, SCORE[score], groups, top_groups, group_best,
                    1 if renormalize else 0, _bits(scale), (torch.int32, tokens, top_k), (torch.float32, tokens, top_k))
 
 
