@@ -85,13 +85,26 @@ int launch(const GemvArgs& a, hipStream_t s) {
     return CMX_OK;
 }
 
+// Two tiles of rows share what a workgroup reads of x, one tile makes twice the workgroups.  Up to 4 rows of x the workgroups matter more (us, bf16 x, weights
+// from memory, one tile / two tiles, N x K: 1 row of x, 4096 x 7168 6.1 / 7.5, 16384 x 8192 18.6 / 20.8; 4 rows, 32768 x 2048 10.4 / 12.0); from 5 rows on
+// two tiles win where they still leave three workgroups to four CUs (8 rows, 16384 x 8192 28.4 / 23.2; 16 rows, 7168 x 2048 7.9 / 5.3, 16384 x 8192
+// 34.6 / 26.0; 64 rows, 4096 x 7168 25.8 / 18.0) and lose where they do not (8 rows, 4096 x 7168 7.6 / 9.5; 16 rows 9.6 / 10.9, 2048 x 16384 14.6 / 18.7).
+// Four tiles spill registers or take too much LDS (16 rows, 16384 x 8192: 44).
+template <int KIND, int COLUMNS>
+int launch_tiles(const GemvArgs& a, hipStream_t s) {
+    int cus;
+    if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
+    if (4 * (uint64_t)ceil_div(a.n, 32) * ceil_div(a.m, COLUMNS) >= 3 * (uint64_t)cus) return launch<KIND, 2, COLUMNS>(a, s);
+    return launch<KIND, 1, COLUMNS>(a, s);
+}
+
 template <int KIND>
 int launch(const GemvArgs& a, hipStream_t s) {
     if (a.m <= 1) return launch<KIND, 1, 1>(a, s);
     if (a.m <= 2) return launch<KIND, 1, 2>(a, s);
     if (a.m <= 4) return launch<KIND, 1, 4>(a, s);
-    if (a.m <= 8 || KIND == kXFp32) return launch<KIND, 1, 8>(a, s);
-    return launch<KIND, 1, KIND == kXFp32 ? 8 : 16>(a, s);
+    if (a.m <= 8 || KIND == kXFp32) return launch_tiles<KIND, 8>(a, s);
+    return launch_tiles<KIND, KIND == kXFp32 ? 8 : 16>(a, s);
 }
 
 }  // namespace

@@ -56,6 +56,17 @@ def test_every_length_of_k(k, x, out):
             check(got, a, wide)
 
 
+@pytest.mark.parametrize("k", [32, 96, 544, 2080, 5120])
+@pytest.mark.parametrize("x,out", [("bf16", "bf16"), ("fp16", "fp16"), ("fp32", "fp32")])
+def test_every_length_of_k_under_many_rows(k, x, out):
+    """Enough weight rows for two tiles of them to a workgroup, the last one in part."""
+    w, s = weights(8209, k, k)
+    wide = dequantized(w, s)
+    for m in (5, 9, 20):
+        a = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(m)).to(DTYPES[x])
+        check(ops.mxfp4_gemv(a, w, s, out), a, wide)
+
+
 @pytest.mark.parametrize("n", [1, 2, 3, 16, 17, 31, 33, 1000, 4096, 4099, 20000])
 @pytest.mark.parametrize("m", [1, 2, 3, 4, 7, 8, 15, 16, 17, 31, 33, 48, 64, 65, 130])
 def test_whole_numbers_are_exact(m, n):
