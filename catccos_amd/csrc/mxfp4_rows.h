@@ -11,7 +11,9 @@
 // different rows) touch 64 pieces, scale bytes and activations as many again.  So everything is loaded as it lies - four rows x 256 bytes of weights,
 // 16 bytes of a row's scales, whole kilobytes of activations - into registers, of which a CU has three times as much as LDS, and changes lanes through a
 // piece of LDS that is the wavefront's own: nothing waits for another wavefront.
-// Measured (FFN of 32 tokens, 163 of 256 experts, K = 7168, N = 4096): CMX_MEASURED
+// Measured (both matmuls of the FFN of 32 tokens, 163 of 256 experts with 3.8 GB of weights, K = 7168, N = 4096; us): loads as the instruction wants them, a
+// scale byte per lane and step, 1541; scales by the word and activations straight to LDS 930; everything as it lies 745.  Of that the first matmul reads
+// at 5.7 TB/s and the second at 4.2; a plain sum over as many bytes reaches 6.2.
 #pragma once
 
 #include "mx_common.h"

@@ -61,6 +61,25 @@ def test_against_the_formula(tokens, e, top_k, k, n):
     check(ops.mxfp4_moe_ffn(x, idx, gate, *w), x, idx, gate, *w)
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 9, 70])
+def test_wide_rows(tokens):
+    """Rows of W2 for two tiles to a workgroup of the second matmul, the last one in part; k is no multiple of a whole step."""
+    w = experts_of(5, 64, 6176, 11)
+    x = torch.randn((tokens, 6176), device="cuda", generator=torch.Generator(device="cuda").manual_seed(tokens)).to(torch.bfloat16)
+    idx, gate = routing(tokens, 5, 2, tokens)
+    check(ops.mxfp4_moe_ffn(x, idx, gate, *w), x, idx, gate, *w)
+
+
+def test_captured_right_after_init():
+    """First launches inside a stream capture, after cmx_init() alone (tests/capture_decode_child.py)."""
+    import os
+    import subprocess
+    import sys
+    child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "capture_decode_child.py")
+    r = subprocess.run([sys.executable, child], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "CAPTURE-OK" in r.stdout, (r.returncode, r.stdout[-2000:], r.stderr[-2000:])
+
+
 def test_many_routes_and_the_widest_top_k():
     w = experts_of(64, 128, 256, 1)
     for tokens in (3, 64, 70):
