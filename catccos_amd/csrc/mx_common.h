@@ -53,6 +53,8 @@ int preload_moe_ffn_kernels();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+// threads of a launch along one axis are counted in 32 bits
+inline bool fits_grid(uint64_t blocks, uint32_t threads) { return blocks * threads < (1ull << 32); }
 inline uint32_t round_up(uint32_t a, uint32_t b) { return ceil_div(a, b) * b; }
 inline size_t round_up_sz(size_t a, size_t b) { return (a + b - 1) / b * b; }
 // scale bytes per row: ceil(cols/32) rounded up to an even count

@@ -125,7 +125,8 @@ extern "C" int cmx_mxfp4_gemv(const void* x, uint32_t ld_x, int x_type, const ui
     CMX_REQUIRE(known(x_type) && known(out_type), "unknown type");
     if (m == 0 || n == 0) return CMX_OK;
     CMX_REQUIRE(x && b && b_scale && out, "null pointer");
-    CMX_REQUIRE(k > 0 && k % 32 == 0, "k must be a positive multiple of 32");
+    CMX_REQUIRE(k > 0 && k % 32 == 0 && k <= (1u << 29), "k must be a positive multiple of 32, at most 2^29");
+    CMX_REQUIRE(n <= (1u << 26), "too many rows of b");
     CMX_REQUIRE(ld_x >= k && ld_b >= k / 2 && ld_bs >= k / 32 && ld_out >= n, "row pitch smaller than row");
     CMX_REQUIRE(aligned16(b) && ld_b % 16 == 0, "weight rows must be 16-byte aligned");
     const uint32_t xb = x_type == CMX_OUT_FP32 ? 4 : 2, ob = out_type == CMX_OUT_FP32 ? 4 : 2;

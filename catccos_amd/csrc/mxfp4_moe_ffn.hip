@@ -323,8 +323,8 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
                                  const uint8_t* w2, const uint8_t* w2_scale, void* out, uint8_t* workspace, uint32_t m, uint32_t k, uint32_t n,
                                  uint32_t experts, uint32_t top_k, cmx_stream_t stream) {
     using namespace cmx;
-    CMX_REQUIRE(k > 0 && k % 32 == 0, "k must be a positive multiple of 32");
-    CMX_REQUIRE(n > 0 && n % 64 == 0, "n must be a positive multiple of 64");
+    CMX_REQUIRE(k > 0 && k % 32 == 0 && k <= (1u << 26), "k must be a positive multiple of 32, at most 2^26");
+    CMX_REQUIRE(n > 0 && n % 64 == 0 && n <= (1u << 26), "n must be a positive multiple of 64, at most 2^26");
     CMX_REQUIRE(experts > 0 && experts < (1u << 31), "experts must be in [1, 2^31)");
     CMX_REQUIRE(top_k > 0 && top_k <= kMaxTopK, "top_k must be in [1, 64]");
     CMX_REQUIRE((uint64_t)m * top_k < (1ull << 31) && m <= 65535u * kTokens, "too many tokens");

@@ -311,17 +311,20 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a) {
 }
 
 template <int TYPE, int WTYPE>
-void launch(const NormArgs& a, hipStream_t s) {
+int launch(const NormArgs& a, hipStream_t s) {
     const auto run = [&](auto kernel, uint32_t rows_each, uint32_t threads) {
+        CMX_REQUIRE(fits_grid(((uint64_t)a.rows + rows_each - 1) / rows_each, threads), "too many rows");
         hipLaunchKernelGGL(kernel, dim3(ceil_div(a.rows, rows_each)), dim3(threads), 0, s, a);
+        CMX_LAUNCH_CHECK();
+        return CMX_OK;
     };
-    if (a.cols <= 512) run(rms_norm_kernel<TYPE, WTYPE, 64, 1>, 4, 256);
-    else if (a.cols <= 1024) run(rms_norm_kernel<TYPE, WTYPE, 64, 2>, 4, 256);
-    else if (a.cols <= 2048) run(rms_norm_kernel<TYPE, WTYPE, 256, 1>, 1, 256);
-    else if (a.cols <= 4096) run(rms_norm_kernel<TYPE, WTYPE, 256, 2>, 1, 256);
-    else if (a.cols <= 8192) run(rms_norm_kernel<TYPE, WTYPE, 256, 4>, 1, 256);
-    else if (a.cols <= 16384) run(rms_norm_kernel<TYPE, WTYPE, 1024, 2>, 1, 1024);
-    else run(rms_norm_long_kernel<TYPE, WTYPE>, 1, 1024);
+    if (a.cols <= 512) return run(rms_norm_kernel<TYPE, WTYPE, 64, 1>, 4, 256);
+    if (a.cols <= 1024) return run(rms_norm_kernel<TYPE, WTYPE, 64, 2>, 4, 256);
+    if (a.cols <= 2048) return run(rms_norm_kernel<TYPE, WTYPE, 256, 1>, 1, 256);
+    if (a.cols <= 4096) return run(rms_norm_kernel<TYPE, WTYPE, 256, 2>, 1, 256);
+    if (a.cols <= 8192) return run(rms_norm_kernel<TYPE, WTYPE, 256, 4>, 1, 256);
+    if (a.cols <= 16384) return run(rms_norm_kernel<TYPE, WTYPE, 1024, 2>, 1, 1024);
+    return run(rms_norm_long_kernel<TYPE, WTYPE>, 1, 1024);
 }
 
 }  // namespace
@@ -361,9 +364,7 @@ extern "C" int cmx_rms_norm_quant(const void* x, uint32_t ld_x, const void* resi
                         static_cast<uint8_t*>(total), static_cast<uint8_t*>(y), codes, scales, (size_t)ld_x * bytes, (size_t)ld_residual * bytes,
                         (size_t)ld_total * bytes, (size_t)ld_y * bytes, ld_codes, ld_scales, rows, cols, eps, fmt};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (type == kBf16) weight_type == kBf16 ? launch<kBf16, kBf16>(a, s) : launch<kBf16, kFp32>(a, s);
-    else if (type == kFp16) weight_type == kFp16 ? launch<kFp16, kFp16>(a, s) : launch<kFp16, kFp32>(a, s);
-    else launch<kFp32, kFp32>(a, s);
-    CMX_LAUNCH_CHECK();
-    return CMX_OK;
+    if (type == kBf16) return weight_type == kBf16 ? launch<kBf16, kBf16>(a, s) : launch<kBf16, kFp32>(a, s);
+    if (type == kFp16) return weight_type == kFp16 ? launch<kFp16, kFp16>(a, s) : launch<kFp16, kFp32>(a, s);
+    return launch<kFp32, kFp32>(a, s);
 }

@@ -117,7 +117,16 @@ def _pitch(t, cols: int) -> int:
         return cols
     pitch, step = t.stride()
     assert step == 1 or cols <= 1, "rows must lie in one piece"
-    return pitch if t.size(0) > 1 else cols
+    if t.size(0) <= 1:
+        return cols
+    _fits(pitch)
+    return pitch
+
+
+def _fits(sizes: int):
+    """Sizes, or'ed together: the entry points take them in 32 bits."""
+    if sizes >> 32:
+        raise ValueError("sizes and pitches must stay below 2^32")
 
 
 def _bits(value) -> int:
@@ -159,6 +168,7 @@ def _norm(x, weight, eps, residual, total, y, codes, scales, code_cols, scale_co
     not the caller's."""
     _here(x, weight, residual, total)
     rows, cols = x.shape
+    _fits(rows | cols)
     dtype = x.dtype
     assert weight.shape == (cols,) and weight.is_contiguous() and (weight.dtype == dtype or weight.dtype == torch.float32)
     r_pitch = t_pitch = cols
@@ -207,6 +217,7 @@ def mxfp4_gemv(x: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: str
     """A few rows x [m, k] bf16 / fp16 / fp32, as they are, times MXFP4 weights b u8 [n, k/2] with b_scale u8 [n, >= k/32] -> [m, n]."""
     _here(x, b, b_scale)
     (m, k), n = x.shape, b.shape[0]
+    _fits(m | n | k)
     assert b.dtype == b_scale.dtype == torch.uint8 and 2 * b.shape[1] == k and b_scale.shape[0] == n and 32 * b_scale.shape[1] >= k
     return _launch("cmx_mxfp4_gemv", x, _pitch(x, k), _TYPE[x.dtype], b, _pitch(b, b.shape[1]), b_scale, _pitch(b_scale, b_scale.shape[1]),
                    (_OUT_DTYPE[out], m, n), n, OUT[out], m, n, k)
@@ -393,6 +404,7 @@ def moe_gating(logits: torch.Tensor, top_k: int, score: str = "softmax", bias=No
     top_k, groups, top_groups, group_best = index(top_k), index(groups), index(top_groups), index(group_best)
     _here(logits, bias)
     tokens, experts = logits.shape
+    _fits(tokens | experts | top_k | groups | top_groups | group_best)
     assert bias is None or (bias.shape == (experts,) and bias.dtype == torch.float32 and bias.is_contiguous())
     return _launch("cmx_moe_gating", logits, _pitch(logits, experts), _TYPE[logits.dtype], bias, tokens, experts, top_k, SCORE[score], groups, top_groups, group_best,
                    1 if renormalize else 0, _bits(scale), (torch.int32, tokens, top_k), (torch.float32, tokens, top_k))
@@ -443,7 +455,9 @@ def moe_token_unpermute(y: torch.Tensor, src2sorted: torch.Tensor, probs: torch.
 
 
 def mxfp4_moe_ffn_workspace_bytes(m: int, n: int, top_k: int) -> int:
-    return _lib.load().cmx_mxfp4_moe_ffn_workspace_bytes(index(m), index(n), index(top_k))
+    m, n, top_k = index(m), index(n), index(top_k)
+    _fits(m | n | top_k)
+    return _lib.load().cmx_mxfp4_moe_ffn_workspace_bytes(m, n, top_k)
 
 
 def mxfp4_moe_ffn(x, expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, workspace=None, out=None) -> torch.Tensor:
@@ -452,6 +466,7 @@ def mxfp4_moe_ffn(x, expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, worksp
     -> bf16 [m, k].  A route to an expert outside [0, E) adds nothing."""
     _here(x, expert_idx, gate_weight, w1, w1_scale, w2, w2_scale, workspace, out)
     (m, k), (e, n), top_k = x.shape, w1.shape[:2], expert_idx.shape[1]
+    _fits(m | k | e | n | top_k)
     assert x.element_size() == 2 and x.dtype != torch.float16 and expert_idx.dtype == torch.int32 and gate_weight.dtype == torch.float32
     assert expert_idx.shape == gate_weight.shape == (m, top_k)
     assert w1.shape == (e, n, k // 2) and w1_scale.shape == (e, n, scale_cols(k)) and w2.shape == (e, k, n // 4) and w2_scale.shape == (e, k, scale_cols(n // 2))

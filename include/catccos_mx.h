@@ -344,7 +344,7 @@ int cmx_int8_gmm_dequant_swiglu(const int8_t* a, uint32_t lda, const float* toke
  *   bias         fp32 [experts] or NULL; it moves the choice, not the weights
  *   scale_bits   scale as the 32 bits of a float
  *   expert_idx   int32 [tokens, top_k], gate_weight fp32 [tokens, top_k]
- * experts <= 1024, groups <= 64 and a divisor of experts, top_k <= 64.  A logit or bias of -Inf masks an expert: it is chosen
+ * tokens < 2^26, experts <= 1024, groups <= 64 and a divisor of experts, top_k <= 64.  A logit or bias of -Inf masks an expert: it is chosen
  * when no other is left.  A row of -Inf has scores of zero.  NaN is chosen like -Inf; a NaN or +Inf in a softmax row makes
  * its weights NaN.  Whatever a row holds, its indices are distinct and in [0, experts).
  * ---------------------------------------------------------------------------------------- */

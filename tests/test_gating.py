@@ -42,3 +42,10 @@ def test_bad_arguments_are_refused_before_a_launch(change, message):
 
 def test_nothing_to_do_is_no_error():
     assert _lib.load().cmx_moe_gating(*{**WHOLE, "tokens": 0, "logits": None}.values()) == 0
+
+
+@pytest.mark.parametrize("tokens", [1 << 26, (1 << 31) - 1])
+def test_more_tokens_than_a_launch_has_threads_for(tokens):
+    lib = _lib.load()
+    assert lib.cmx_moe_gating(*{**WHOLE, "tokens": tokens, "top_k": 1}.values()) == -1
+    assert b"below 2^26" in lib.cmx_last_error()

@@ -30,3 +30,22 @@ def test_bad_arguments_are_refused_before_a_launch(change, message):
 @pytest.mark.parametrize("change", [dict(m=0), dict(n=0), dict(m=0, x=None)])
 def test_nothing_to_do_is_no_error(change):
     assert _lib.load().cmx_mxfp4_gemv(*{**WHOLE, **change}.values()) == 0
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(n=(1 << 26) + 16, ld_out=1 << 27), "too many rows of b"), (dict(n=0xFFFFFFF0, ld_out=0xFFFFFFFF), "too many rows of b"),
+    (dict(k=1 << 30, ld_x=1 << 30, ld_b=1 << 29, ld_bs=1 << 25), "at most 2^29")])
+def test_sizes_that_32_bits_of_a_launch_cannot_hold(change, message):
+    test_bad_arguments_are_refused_before_a_launch(change, message)
+
+
+def test_pitches_and_sizes_past_32_bits_are_refused_in_front():
+    far = torch.empty_strided((2, 64), (1 << 32, 1), dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="2\\^32"):
+        ops._pitch(far, 64)
+    assert ops._pitch(far[:1], 64) == 64                              # (the stride of a single row says nothing)
+    for call in (lambda: ops._fits(1 << 32), lambda: ops._fits(5 | -3), lambda: ops.mxfp4_moe_ffn_workspace_bytes(1 << 32, 64, 1),
+                 lambda: ops.mxfp4_moe_ffn_workspace_bytes(1, 64, -1)):
+        with pytest.raises(ValueError, match="2\\^32"):
+            call()
+    ops._fits((1 << 32) - 1)

@@ -34,3 +34,8 @@ def test_no_tokens_and_the_workspace():
     need = ops.mxfp4_moe_ffn_workspace_bytes(32, 4096, 8)
     assert need >= 256 * 2048 * 4 and need % 256 == 0
     assert ops.mxfp4_moe_ffn_workspace_bytes(1 << 20, 4096, 8) >= (1 << 23) * 2048 * 4          # past 32 bits
+
+
+@pytest.mark.parametrize("change,message", [(dict(k=(1 << 26) + 32), "at most 2^26"), (dict(n=(1 << 26) + 64), "at most 2^26"), (dict(n=0xFFFFFFC0), "at most 2^26")])
+def test_sizes_that_32_bits_of_a_launch_cannot_hold(change, message):
+    test_bad_arguments_are_refused_before_a_launch(change, message)

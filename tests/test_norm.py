@@ -51,3 +51,11 @@ def test_nothing_to_do_is_no_error(change):
 def test_eps_as_bits():
     assert ops._bits(1.0) == 0x3F800000 and ops._bits(0.0) == 0
     assert ops._bits(1e300) == 0x7F800000                         # (which the entry point refuses)
+
+
+@pytest.mark.parametrize("rows,cols", [((1 << 26) + 1, 1), (0xFFFFFFFF, 1), (1 << 24, 1040), (1 << 22, 8200), (1 << 22, 20000)])
+def test_more_rows_than_a_launch_has_threads_for(rows, cols):
+    lib = _lib.load()
+    pitch = 20000
+    assert lib.cmx_rms_norm_quant(*{**WHOLE, "rows": rows, "cols": cols, **{name: pitch for name in WHOLE if name.startswith("ld_")}}.values()) == -1
+    assert b"too many rows" in lib.cmx_last_error()
