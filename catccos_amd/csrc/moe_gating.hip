@@ -382,19 +382,28 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
                 const uint32_t g = expert(s) * a.by_members >> 20;
                 if ((lane & (over - 1)) == 0 && g < a.groups) enter(g, first, second);
             }
-        } else {                                                        // groups of other sizes: a lane for each
+        } else {                                                        // groups of other sizes: as many lanes for each as there are, a power of two
 #pragma unroll
             for (int s = 0; s < SLOTS; ++s) ords[expert(s)] = o[s];
             __builtin_amdgcn_wave_barrier();
-            for (uint32_t g = lane; g < a.groups; g += LPR) {
-                uint32_t first = 0, second = 0, j = g % a.members;      // (each lane starts elsewhere: no two read one bank)
-                for (uint32_t n = 0; n < a.members; ++n) {
-                    const uint32_t v = ords[g * a.members + j];
-                    j = j + 1 == a.members ? 0 : j + 1;
-                    second = max(second, min(first, v));
-                    first = max(first, v);
-                }
-                enter(g, first, second);
+            uint32_t team = LPR;
+            while (team > 1 && team * a.groups > (uint32_t)LPR) team >>= 1;
+            for (uint32_t g0 = 0; g0 < a.groups; g0 += LPR / team) {
+                const uint32_t g = g0 + lane / team;
+                uint32_t first = 0, second = 0;
+                const auto join = [&](uint32_t f, uint32_t g) {
+                    second = max(max(second, g), min(first, f));
+                    first = max(first, f);
+                };
+                if (g < a.groups)
+                    for (uint32_t j = lane & (team - 1); j < a.members; j += team) join(ords[g * a.members + j], 0);
+                if (team > 1) join(dpp<0xB1>(first), dpp<0xB1>(second));
+                if (team > 2) join(dpp<0x4E>(first), dpp<0x4E>(second));
+                if (team > 4) join(dpp<0x141>(first), dpp<0x141>(second));
+                if (team > 8) join(dpp<0x140>(first), dpp<0x140>(second));
+                if (LPR == 64 && team > 16) join((uint32_t)__shfl_xor((int)first, 16), (uint32_t)__shfl_xor((int)second, 16));
+                if (LPR == 64 && team > 32) join((uint32_t)__shfl_xor((int)first, 32), (uint32_t)__shfl_xor((int)second, 32));
+                if ((lane & (team - 1)) == 0 && g < a.groups) enter(g, first, second);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -562,7 +571,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
         border = row_bits(__ballot(border)) != 0;
         tied = border && row_bits(__ballot(tied)) != 0;
         near |= border && row_bits(__ballot(open)) != 0;
-        near |= mend && (tied || a.top_k + 1 > (uint32_t)LPR);
+        near |= mend && (tied || min(a.top_k + 1, rounds) > (uint32_t)LPR);
         if (tied && !mend) {
             const float zl = scores[a.top_k].x, sl = scores[a.top_k].y, bl = bias(picks[a.top_k].x);
 #pragma unroll
@@ -670,13 +679,15 @@ extern "C" int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, 
         else if (slots <= 2) run(lanes, integral_constant<int, 2>());
         else if (slots <= 4) run(lanes, integral_constant<int, 4>());
         else if (slots <= 8) run(lanes, integral_constant<int, 8>());
-        else run(lanes, integral_constant<int, 16>());
+        else if (slots <= 16 || lanes.value == 64) run(lanes, integral_constant<int, 16>());
+        else run(lanes, integral_constant<int, lanes.value == 16 ? 32 : 16>());
     };
     // 16 lanes to a row do less work, 64 are done sooner.  Measured in a graph, 64 and 16 lanes, softmax top-8 of 256 / sigmoid in 8 groups: 1024 rows 5.3 and
-    // 6.0 / 7.0 and 9.9 us, 3072 rows 6.3 and 6.1 / 8.7 and 10.1, 4096 rows 7.1 and 6.2 / 10.9 and 10.0, on 256 CUs.
+    // 6.0 / 7.0 and 9.9 us, 3072 rows 6.3 and 6.1 / 8.7 and 10.1, 4096 rows 7.1 and 6.2 / 10.9 and 10.0, on 256 CUs; of 512, 4096 rows 10.5 and 10.0 / 14.9 and 15.3, 32768
+    // rows 43.6 and 28.4 / 63.5 and 43.1.
     int cus;
     if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
-    if (tokens >= 14u * (uint32_t)cus && experts <= 256) by_slots(integral_constant<int, 16>());
+    if (tokens >= 14u * (uint32_t)cus && experts <= 512) by_slots(integral_constant<int, 16>());
     else by_slots(integral_constant<int, 64>());
     CMX_LAUNCH_CHECK();
     return CMX_OK;

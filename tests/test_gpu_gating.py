@@ -195,3 +195,15 @@ def test_into_the_routing_sort():
     assert torch.equal(counts.long(), torch.bincount(idx.flatten().long(), minlength=256))
     assert torch.equal(order.long(), idx.flatten().long().sort(stable=True).indices)
     assert bool(((w.sum(dim=1) - 1).abs() < 1e-5).all())
+
+
+@pytest.mark.parametrize("tokens", [37, 3700])
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [(434, 2, 1, 4), (272, 4, 4, 1), (230, 2, 2, 11), (500, 10, 3, 8), (66, 33, 9, 16), (448, 64, 20, 8), (1000, 5, 2, 9),
+                                                              (512, 1, 1, 8), (512, 8, 4, 16), (32, 2, 1, 16), (45, 15, 7, 3)])
+def test_groups_of_every_size_and_many_experts(tokens, experts, groups, top_groups, top_k):
+    """Groups that do not fall on whole lanes, more of them than a row has lanes, more experts than a row has by the lane; few rows and many."""
+    g = torch.Generator(device="cuda").manual_seed(experts + tokens)
+    for dtype, score, group_best in ((torch.float32, "softmax", 1), (torch.float16, "sigmoid", 2), (torch.bfloat16, "softmax", 2)):
+        z = torch.randn((tokens, experts), generator=g, device="cuda").to(dtype)
+        for bias in (None, 0.1 * torch.randn(experts, generator=g, device="cuda")):
+            _check(z, top_k, score, bias, groups, top_groups, group_best)
