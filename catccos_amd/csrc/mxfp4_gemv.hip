@@ -102,11 +102,20 @@ int launch_tiles(const GemvArgs& a, hipStream_t s) {
 
 template <int KIND>
 int launch(const GemvArgs& a, hipStream_t s) {
-    if (a.m <= 1) return launch<KIND, 1, 1>(a, s);
-    if (a.m <= 2) return launch<KIND, 1, 2>(a, s);
-    if (a.m <= 4) return launch<KIND, 1, 4>(a, s);
-    if (a.m <= 8 || KIND == kXFp32) return launch_tiles<KIND, 8>(a, s);
-    return launch_tiles<KIND, KIND == kXFp32 ? 8 : 16>(a, s);
+    constexpr uint32_t kMost = KIND == kXFp32 ? 8 : 16;
+    int cus;
+    if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
+    uint32_t columns = 1;
+    while (columns < kMost && columns < a.m) columns *= 2;
+    // A long K under few weight rows: workgroups that share a weight row's tile have fewer columns each, which costs them less time than the CUs stood idle
+    // (K > 4096; 16 columns / as many as leave a workgroup to a CU, 16 rows of x: 127 x 15584 bf16 11.7 / 7.1 us, fp16 21.7 / 9.1, fp32 26.5 / 10.8,
+    // 728 x 11424 bf16 10.8 / 7.4; up to K = 4096 a wavefront has one unit and nothing is gained: 1756 x 896 3.9 / 4.3).
+    while (columns > 1 && a.blocks > 8 * kUnitBlocks && (uint64_t)ceil_div(a.n, 16) * ceil_div(a.m, columns / 2) <= (uint32_t)cus) columns /= 2;
+    if (columns <= 1) return launch<KIND, 1, 1>(a, s);
+    if (columns <= 2) return launch<KIND, 1, 2>(a, s);
+    if (columns <= 4) return launch<KIND, 1, 4>(a, s);
+    if (columns <= 8 || kMost == 8) return launch_tiles<KIND, 8>(a, s);
+    return launch_tiles<KIND, kMost>(a, s);
 }
 
 }  // namespace

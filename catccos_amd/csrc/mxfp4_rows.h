@@ -22,6 +22,7 @@ namespace cmx {
 
 typedef __bf16 v8bf16 __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kUnitSteps = 4, kUnitBlocks = 16, kUnitK = 512;        // a step: four blocks of 32 along K, one for each 16 lanes
 
@@ -34,8 +35,18 @@ struct XTraits {
     static constexpr int kPieces = KIND == kXBf16 ? 1 : (KIND == kXFp32 ? 3 : 2);
     static constexpr uint32_t kBytes = KIND == kXFp32 ? 4 : 2;                     // of an element, in one array
     static constexpr int kReads = KIND == kXFp32 || KIND == kXPlanes ? 2 : 1;      // 16-byte pieces that hold eight values
-    static constexpr uint32_t kPitch = kReads * 1024 + 16;                         // of a column in LDS: a unit of one row of x
 };
+// Whether fp16 and fp32 are taken to pieces on their way into LDS, once for each value, or behind it, by each lane that takes it: a tile's 16 columns are
+// COLUMNS rows of x again and again.  Pieces take more of LDS than the value, which costs wavefronts where columns are many.  (Matrix-vector product,
+// 4096 x 7168, us, behind LDS and before: fp16, 1 row 10.8 and 7.0, 8 rows 12.2 and 10.1; fp32, 1 row 13.4 and 8.1, 8 rows 16.4 and 14.5.)
+template <int KIND, int COLUMNS>
+constexpr bool kPiecesInLds = KIND == kXPlanes || KIND == kXFp32 || (KIND == kXFp16 && COLUMNS <= 8);
+// 16-byte parts of LDS that hold eight values: of each piece, or of the value
+template <int KIND, int COLUMNS>
+constexpr int kParts = kPiecesInLds<KIND, COLUMNS> ? XTraits<KIND>::kPieces : XTraits<KIND>::kReads;
+// bytes of a column in LDS: a unit of one row of x
+template <int KIND, int COLUMNS>
+constexpr uint32_t kColumnPitch = kParts<KIND, COLUMNS> * 1024 + 16;
 
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
 // ---- weights --------------------------------------------------------------------------------------------------------
@@ -60,7 +71,7 @@ constexpr uint32_t kRowPitch = 256 + 16;        // of a weight row in LDS
 
 // Bytes of LDS of a wavefront: a unit of RT x 16 weight rows, 16 bytes of scales for each, COLUMNS columns of activations
 template <int KIND, int RT, int COLUMNS>
-constexpr uint32_t kStageBytes = RT * (16 * kRowPitch + 256) + COLUMNS * XTraits<KIND>::kPitch;
+constexpr uint32_t kStageBytes = RT * (16 * kRowPitch + 256) + COLUMNS * kColumnPitch<KIND, COLUMNS>;
 
 // RT x 16 weight rows times up to COLUMNS (1 to 16) activation rows.
 //
@@ -69,6 +80,9 @@ constexpr uint32_t kStageBytes = RT * (16 * kRowPitch + 256) + COLUMNS * XTraits
 template <int KIND, int RT, int COLUMNS, bool STREAM>
 struct RowsStream {
     using T = XTraits<KIND>;
+    static constexpr bool kInPieces = kPiecesInLds<KIND, COLUMNS>;
+    static constexpr int kPartsOf = kParts<KIND, COLUMNS>;
+    static constexpr uint32_t kPitch = kColumnPitch<KIND, COLUMNS>;
     // a lane's own: where its 16 bytes of each group of four weight rows and its four of the scales come from, at K = 0
     const uint8_t *a[RT][4], *scale[RT];
     uint32_t blocks;           // K / 32
@@ -146,19 +160,39 @@ struct RowsStream {
             for (int g = 0; g < 4; ++g) *(lds4)(uintptr_t)(stage + (i * 16 + g * 4 + lane / 16) * kRowPitch + lane % 16 * 16) = u.a[i][g];
         }
 #pragma unroll
-        for (int c = 0; c < COLUMNS; ++c)
+        for (int c = 0; c < COLUMNS; ++c) {
+            const uint32_t to = xs + c * kPitch + lane * 16;
+            if constexpr (!kInPieces || KIND == kXPlanes) {
 #pragma unroll
-            for (int l = 0; l < T::kReads; ++l) *(lds4)(uintptr_t)(xs + c * T::kPitch + l * 1024 + lane * 16) = u.x[c][l];
+                for (int l = 0; l < T::kReads; ++l) *(lds4)(uintptr_t)(to + l * 1024) = u.x[c][l];
+            } else if constexpr (KIND == kXFp16) {
+                v8bf16 piece[T::kPieces];
+                operands(&u.x[c][0], piece);
+#pragma unroll
+                for (int n = 0; n < T::kPieces; ++n) *(lds4)(uintptr_t)(to + n * 1024) = __builtin_bit_cast(v4u, piece[n]);
+            } else {
+                typedef __attribute__((address_space(3))) v2u* lds2;      // (four of the eight values from each half of the unit)
+                v8bf16 piece[T::kPieces];
+                operands(&u.x[c][0], piece);
+#pragma unroll
+                for (int n = 0; n < T::kPieces; ++n) {
+                    const v4u w = __builtin_bit_cast(v4u, piece[n]);
+                    *(lds2)(uintptr_t)(to - lane * 8 + n * 1024) = (v2u){w.x, w.y};
+                    *(lds2)(uintptr_t)(to - lane * 8 + n * 1024 + 512) = (v2u){w.z, w.w};
+                }
+            }
+        }
     }
 
     // what a lane takes from LDS for one step
     struct Step {
-        v4u codes[RT], x[4][T::kReads];
+        v4u codes[RT], x[4][kPartsOf];
         uint32_t scale[RT];
     };
     __device__ __forceinline__ void read(Step& g, uint32_t xs, int s) const {
         typedef const __attribute__((address_space(3))) v4u* lds4;
         typedef const __attribute__((address_space(3))) uint8_t* lds1;
+        constexpr uint32_t kBytes = kInPieces ? 2 : T::kBytes;
         const uint32_t r = threadIdx.x & 15, q = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -168,15 +202,14 @@ struct RowsStream {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int l = 0; l < T::kReads; ++l)
-                g.x[j][l] = *(lds4)(uintptr_t)(xs + q * (32 * T::kBytes) + s * (128 * T::kBytes) + j * (8 * T::kBytes) + l * (KIND == kXPlanes ? 1024 : 16));
+            for (int l = 0; l < kPartsOf; ++l)
+                g.x[j][l] = *(lds4)(uintptr_t)(xs + q * (32 * kBytes) + s * (128 * kBytes) + j * (8 * kBytes) + l * 1024);
     }
     // eight activations as kPieces operands.  A value is the sum of its pieces, exactly: each takes the leading eight bits of what is left.
-    __device__ __forceinline__ static void operands(const v4u (&x)[T::kReads], v8bf16 (&out)[T::kPieces]) {
-        if constexpr (KIND == kXBf16 || KIND == kXPlanes) {
-#pragma unroll
-            for (int n = 0; n < T::kPieces; ++n) out[n] = __builtin_bit_cast(v8bf16, x[n]);
-        } else {
+    __device__ __forceinline__ static void operands(const v4u* x, v8bf16 (&out)[T::kPieces]) {
+        if constexpr (KIND == kXBf16) {
+            out[0] = __builtin_bit_cast(v8bf16, x[0]);
+        } else if constexpr (KIND != kXPlanes) {
             float v[8];
             if constexpr (KIND == kXFp16) {
                 typedef _Float16 v8f16 __attribute__((ext_vector_type(8)));
@@ -208,7 +241,7 @@ struct RowsStream {
     // the unit in LDS, onto acc
     template <bool WHOLE>
     __device__ __forceinline__ void multiply(uint32_t unit) {
-        const uint32_t q = (threadIdx.x & 63) >> 4, xs = stage + RT * (16 * kRowPitch + 256) + (threadIdx.x & 15) % COLUMNS * T::kPitch;      // (columns again and again)
+        const uint32_t q = (threadIdx.x & 63) >> 4, xs = stage + RT * (16 * kRowPitch + 256) + (threadIdx.x & 15) % COLUMNS * kPitch;      // (columns again and again)
 #pragma unroll
         for (int s = 0; s < (int)kUnitSteps; ++s) {
             Step g;
@@ -222,7 +255,7 @@ struct RowsStream {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int l = 0; l < T::kReads; ++l) g.x[j][l] = (v4u){0, 0, 0, 0};
+                    for (int l = 0; l < kPartsOf; ++l) g.x[j][l] = (v4u){0, 0, 0, 0};
             }
             float f[RT];
 #pragma unroll
@@ -230,7 +263,12 @@ struct RowsStream {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 v8bf16 v[T::kPieces];
-                operands(g.x[j], v);
+                if constexpr (kInPieces) {
+#pragma unroll
+                    for (int n = 0; n < T::kPieces; ++n) v[n] = __builtin_bit_cast(v8bf16, g.x[j][n]);
+                } else {
+                    operands(g.x[j], v);
+                }
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
                     const v4u c = g.codes[i];

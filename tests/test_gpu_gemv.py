@@ -67,6 +67,17 @@ def test_every_length_of_k_under_many_rows(k, x, out):
         check(ops.mxfp4_gemv(a, w, s, out), a, wide)
 
 
+@pytest.mark.parametrize("n,k", [(5, 4128), (130, 15616), (700, 4640), (2000, 5152)])
+@pytest.mark.parametrize("x,out", [("bf16", "fp32"), ("fp16", "fp32"), ("fp32", "fp32")])
+def test_long_rows_of_few_weights(n, k, x, out):
+    """K long and weight rows few: the rows of x are spread over more workgroups, one or a few to each."""
+    w, s = weights(n, k, k)
+    wide = dequantized(w, s)
+    for m in (1, 3, 7, 8, 12, 33):
+        a = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(m)).to(DTYPES[x])
+        check(ops.mxfp4_gemv(a, w, s, out), a, wide)
+
+
 @pytest.mark.parametrize("n", [1, 2, 3, 16, 17, 31, 33, 1000, 4096, 4099, 20000])
 @pytest.mark.parametrize("m", [1, 2, 3, 4, 7, 8, 15, 16, 17, 31, 33, 48, 64, 65, 130])
 def test_whole_numbers_are_exact(m, n):
