@@ -341,11 +341,15 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
     hipStream_t s = static_cast<hipStream_t>(stream);
     int cus;
     if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
-    a.pass = m < kTokens ? m : kTokens;
-    // The second matmul's workgroups are few where k is small: then its tokens are spread over more of them (45 tokens, 16 experts, k = 992: 25 us with one
-    // pass, 17.9 with two, 17.4 with four).
-    a.down_pass = a.pass;
-    while (a.down_pass > 16 && ceil_div(k, 16) * ceil_div(m, a.down_pass) * 4 < (uint32_t)cus * 3) a.down_pass = ceil_div(a.down_pass, 2);
+    // The second matmul's workgroups are few where k is small: then its tokens are spread over more of them, as long as there are CUs for all (12 tokens, 256
+    // experts, k = 352: 42 us for both matmuls with one pass, 21 with six; 61 tokens, 8 experts, k = 512: 58 with four passes, 46 with eight).
+    a.down_pass = ceil_div(m, ceil_div(m, kTokens));
+    uint32_t halved = 0;
+    while (a.down_pass > 1 && (uint64_t)ceil_div(k, 16) * ceil_div(m, ceil_div(a.down_pass, 2)) <= (uint32_t)cus) {
+        a.down_pass = ceil_div(a.down_pass, 2);
+        ++halved;
+    }
+    a.pass = a.down_pass << halved;
     const uint32_t passes = ceil_div(m, a.pass), tokens = a.pass, most = tokens * top_k;
     // (a workgroup that stands for no expert or for another's is started and ended for nothing; 45 tokens of 3 routes, 16 experts: 17.6 us by route, 10.8 by expert)
     a.by_expert = experts <= most;
@@ -372,22 +376,26 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
         CMX_LAUNCH_CHECK();
         return CMX_OK;
     };
-    // Columns: as many routes as most experts have; what the others have more costs another reading of their weights.  Routes spread at random, one for
-    // each of 256 experts on average: 88 % of those that have any have at most two and 97 % three.
+    // Columns: as many routes as most experts have; what the others have more costs another reading of their weights, and columns that stand empty cost
+    // wavefronts.  Routes spread at random, one for each of 256 experts on average: 88 % of those that have any have at most two and 97 % three.  (90 tokens of 3
+    // routes, 64 experts: 74 us with 16 columns in the first matmul, 63 with 8; 64 tokens of 6, 64 experts, in two passes: 103 us with 8 columns in the
+    // second, 95 with 4; 28 tokens of 3, 16 experts, one pass: 40 and 45.)
+    const auto per_expert = [&](uint32_t routes, uint32_t by) { return routes <= (uint64_t)by * experts; };
+    const uint32_t up_columns = per_expert(most, 2) && tokens > 3 ? 3 : (per_expert(most, 5) && tokens > 8 ? 8 : tokens);
     int rc;
-    const uint32_t up_columns = most <= 2ull * experts && tokens > 3 ? 3 : tokens;
     if (up_columns <= 1) rc = up(std::integral_constant<int, 1>());
     else if (up_columns <= 3) rc = up(std::integral_constant<int, 3>());
     else if (up_columns <= 8) rc = up(std::integral_constant<int, 8>());
     else rc = up(std::integral_constant<int, 16>());
     if (rc != CMX_OK) return rc;
-    // two row tiles share a reading of the activations from LDS, if that leaves workgroups for three CUs of four (32 tokens, 256 experts, k = 7168: 303 us
-    // and 358 with one; 45 tokens in one pass, 16 experts, k = 992: 36 and 25)
     const auto rows = [&](auto rt) -> int {
-        const uint32_t down_columns = down_most <= 2ull * experts && a.down_pass > 2 ? 2 : a.down_pass;
+        const uint32_t down_columns = per_expert(down_most, 2) && a.down_pass > 2 ? 2 : (per_expert(down_most, 4) && a.down_pass > 4 ? 4 : a.down_pass);
         if (down_columns <= 1) return down(rt, std::integral_constant<int, 1>());
         if (down_columns <= 2) return down(rt, std::integral_constant<int, 2>());
+        if (down_columns <= 4) return down(rt, std::integral_constant<int, 4>());
         return down(rt, std::integral_constant<int, 8>());
     };
-    return ceil_div(k, 32) * 4 >= (uint32_t)cus * 3 ? rows(std::integral_constant<int, 2>()) : rows(std::integral_constant<int, 1>());
+    // Two row tiles share a reading of the activations from LDS, if that leaves workgroups for half of the CUs (32 tokens, 256 experts, k = 7168: 303 us
+    // and 358 with one; 31 tokens, 16 experts, k = 4992, both matmuls: 120 and 145; 64 tokens, 64 experts, k = 2048: 128 and 105).
+    return ceil_div(k, 32) * 2 >= (uint32_t)cus ? rows(std::integral_constant<int, 2>()) : rows(std::integral_constant<int, 1>());
 }
