@@ -6,8 +6,10 @@
 // once: its elements stay in registers between the sum of squares and the scaling (a row that is too long for the registers of one
 // workgroup is read twice, the second time mostly from the caches).
 // Work split: a thread holds pieces of eight consecutive elements, so that four neighbouring lanes hold one MX block, whose
-// maximum is then two DPP exchanges away.
-#include "mx_common.h"
+// maximum is then two DPP exchanges away.  Short rows are a wavefront's, which needs no barrier, longer ones a workgroup's.
+// Bound by memory.  With a residual, total and codes of bf16 rows: 8192 x 7168 in 78 us (5.3 TB/s; a plain copy reaches 5.2), of 4096 columns to
+// bf16 6.4 TB/s; rows of odd length, whose pieces lie across cache lines, 3.6 to 4.1.  A single row takes 3.1 us, of which 2.5 are the launch's.
+#include "mx_launch.h"
 
 namespace cmx {
 namespace {
@@ -313,14 +315,22 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a) {
 template <int TYPE, int WTYPE>
 int launch(const NormArgs& a, hipStream_t s) {
     const auto run = [&](auto kernel, uint32_t rows_each, uint32_t threads) {
-        CMX_REQUIRE(fits_grid(((uint64_t)a.rows + rows_each - 1) / rows_each, threads), "too many rows");
         hipLaunchKernelGGL(kernel, dim3(ceil_div(a.rows, rows_each)), dim3(threads), 0, s, a);
         CMX_LAUNCH_CHECK();
         return CMX_OK;
     };
     if (a.cols <= 512) return run(rms_norm_kernel<TYPE, WTYPE, 64, 1>, 4, 256);
     if (a.cols <= 1024) return run(rms_norm_kernel<TYPE, WTYPE, 64, 2>, 4, 256);
-    if (a.cols <= 2048) return run(rms_norm_kernel<TYPE, WTYPE, 256, 1>, 1, 256);
+    if (a.cols <= 2048) {
+        // A wavefront or a workgroup to a row of 16 bits: the former waits for nobody, the latter has shorter rows.  us with codes, 1348 columns: 1024 rows 8.8
+        // and 7.9, 5041 rows 15.6 and 18.6, 32768 rows 77 and 103; 2048 columns, 32768 rows 88 and 93 (of 32 bits 169 and 158).
+        if constexpr (TYPE != kFp32) {
+            int cus;
+            if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
+            if (a.rows >= 16u * (uint32_t)cus) return run(rms_norm_kernel<TYPE, WTYPE, 64, 4>, 4, 256);
+        }
+        return run(rms_norm_kernel<TYPE, WTYPE, 256, 1>, 1, 256);
+    }
     if (a.cols <= 4096) return run(rms_norm_kernel<TYPE, WTYPE, 256, 2>, 1, 256);
     if (a.cols <= 8192) return run(rms_norm_kernel<TYPE, WTYPE, 256, 4>, 1, 256);
     if (a.cols <= 16384) return run(rms_norm_kernel<TYPE, WTYPE, 1024, 2>, 1, 1024);
@@ -360,6 +370,7 @@ extern "C" int cmx_rms_norm_quant(const void* x, uint32_t ld_x, const void* resi
     CMX_REQUIRE(!off(x, bytes) && !off(residual, bytes) && !off(total, bytes) && !off(y, bytes) && !off(weight, weight_type == kFp32 ? 4 : 2),
                 "pointers must be aligned to their elements");
     CMX_REQUIRE(cols <= (1u << 30), "row too long");
+    CMX_REQUIRE(fits_grid((uint64_t)rows + 3, cols <= 1024 ? 64 : (cols <= 8192 ? 256 : 1024)), "too many rows");      // (+ 3: a workgroup of four rows)
     const NormArgs a = {static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(residual), static_cast<const uint8_t*>(weight),
                         static_cast<uint8_t*>(total), static_cast<uint8_t*>(y), codes, scales, (size_t)ld_x * bytes, (size_t)ld_residual * bytes,
                         (size_t)ld_total * bytes, (size_t)ld_y * bytes, ld_codes, ld_scales, rows, cols, eps, fmt};

@@ -212,3 +212,17 @@ def test_on_a_side_stream_and_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, ops.rms_norm_quant(a, weight, residual=r, want_y=True))), rep
+
+
+@pytest.mark.parametrize("x,w,residual", [("bf16", "bf16", True), ("fp16", "fp32", False), ("fp32", "fp32", True)])
+@pytest.mark.parametrize("cols", [1025, 1348, 1600, 2041, 2048])
+def test_many_rows_of_middling_length(cols, x, w, residual):
+    """Rows of 16 bits of which there are many: a wavefront to each."""
+    from catccos_amd import ops
+    a, r, weight = _inputs(5003, cols, x, w, residual, cols)
+    t, y = _definition(a, r, weight, 1e-6)
+    codes, scales, got, total = ops.rms_norm_quant(a, weight, residual=r, want_y=True)
+    _assert_rounded(got, y, "y")
+    _assert_codes(codes, scales, y, "E4M3")
+    if residual:
+        assert torch.equal(total, (a.float() + r.float()).to(a.dtype))
