@@ -653,7 +653,7 @@ extern "C" int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, 
     CMX_REQUIRE(top_groups > 0 && top_groups <= groups, "top_groups must be in [1, groups]");
     CMX_REQUIRE(group_best == 1 || group_best == 2, "group_best must be 1 or 2");
     CMX_REQUIRE(top_k > 0 && top_k <= kMaxTopK && top_k <= top_groups * (experts / groups), "top_k must not exceed 64 or the experts of the chosen groups");
-    CMX_REQUIRE((uint64_t)tokens * top_k < (1ull << 31) && fits_grid(tokens, 64), "tokens must stay below 2^26, tokens * top_k below 2^31 routes");
+    CMX_REQUIRE((uint64_t)tokens * top_k < (1ull << 31) && fits_grid((uint64_t)tokens + 3, 64), "tokens must stay below 2^26, tokens * top_k below 2^31 routes");
     float scale;
     __builtin_memcpy(&scale, &scale_bits, 4);
     CMX_REQUIRE(scale - scale == 0.0f, "scale must be a finite number");

@@ -18,11 +18,14 @@ namespace {
 
 constexpr uint32_t kTokens = 64;         // of one pass over the weights; more tokens are taken in several
 constexpr uint32_t kMaxTopK = 64, kNone = ~0u;
-constexpr uint32_t kDownWaves = 8, kMaxLds = 159 * 1024;
+constexpr uint32_t kMaxLds = 159 * 1024;
 // First matmul, by the columns of a wavefront: small workgroups, three of which share a CU, so that one works while another starts or ends (32 tokens, 256
 // experts: 445 us; one of eight wavefronts 514; one token 24 us and 35); with many columns LDS has room for one (45 tokens, 16 experts, K = 992: 11 us; of
 // four wavefronts 16).
 constexpr uint32_t up_waves(int columns) { return columns <= 4 ? 4 : 8; }
+// Second matmul: as many as registers allow (45 tokens, 128 experts, k = 736: 36.6 us for both matmuls with 8, 35.0 with 12; 90 tokens, 64 experts, k = 576: 68.8 and
+// 63.8).
+constexpr uint32_t down_waves(int row_tiles, int columns) { return row_tiles == 1 && columns <= 4 ? 12 : 8; }
 constexpr uint32_t kEnoughWaves = 1024;          // of the first matmul, below which K is shared out (45 tokens, 16 experts, K = 992: 11 us, unshared 13; one token, 8 experts,
                                                  // K = 7168, that has 1024: 24 us, shared further 28)
 
@@ -161,7 +164,7 @@ __global__ __launch_bounds__(64 * up_waves(COLUMNS), COLUMNS <= 4 ? 3 : 2) void 
 
 // RT x 16 rows of every W2
 template <int RT, int COLUMNS>
-__global__ __launch_bounds__(64 * kDownWaves) void mxfp4_moe_down_kernel(const FfnArgs a) {
+__global__ __launch_bounds__(64 * down_waves(RT, COLUMNS)) void mxfp4_moe_down_kernel(const FfnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // a stage for each wavefront; sums: [wavefront][token][RT * 16 rows]; lists
     __shared__ uint32_t experts_named;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -370,7 +373,7 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
     const uint32_t down_most = a.down_pass * top_k;
     const auto down = [&](auto rt, auto c) -> int {
         const uint32_t each = kStageBytes<kXPlanes, rt.value, c.value> + a.down_pass * 64 * rt.value, lists = down_most * 10 + 16;
-        const uint32_t fit = (kMaxLds - lists) / each, waves = fit < kDownWaves ? fit : kDownWaves;
+        const uint32_t fit = (kMaxLds - lists) / each, most_waves = down_waves(rt.value, c.value), waves = fit < most_waves ? fit : most_waves;
         if (int rc = allow_dynamic_lds<mxfp4_moe_down_kernel<rt.value, c.value>, kMaxLds>(); rc != CMX_OK) return rc;
         hipLaunchKernelGGL((mxfp4_moe_down_kernel<rt.value, c.value>), dim3(ceil_div(k, 16 * rt.value), ceil_div(m, a.down_pass)), dim3(64 * waves), waves * each + lists, s, a);
         CMX_LAUNCH_CHECK();
@@ -395,7 +398,8 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
         if (down_columns <= 4) return down(rt, std::integral_constant<int, 4>());
         return down(rt, std::integral_constant<int, 8>());
     };
-    // Two row tiles share a reading of the activations from LDS, if that leaves workgroups for half of the CUs (32 tokens, 256 experts, k = 7168: 303 us
-    // and 358 with one; 31 tokens, 16 experts, k = 4992, both matmuls: 120 and 145; 64 tokens, 64 experts, k = 2048: 128 and 105).
-    return ceil_div(k, 32) * 2 >= (uint32_t)cus ? rows(std::integral_constant<int, 2>()) : rows(std::integral_constant<int, 1>());
+    // Two row tiles share a reading of the activations from LDS, if that leaves workgroups for more than half of the CUs (both matmuls, two tiles and one: 32 tokens,
+    // 256 experts, k = 7168 714 us and 774; 12 tokens, 64 experts, k = 5120 195 and 203; 31 tokens, 16 experts, k = 4992 126 and 146; 20 tokens, 128
+    // experts, k = 4096 158 and 124).
+    return ceil_div(k, 32) * 16 >= 9 * (uint32_t)cus ? rows(std::integral_constant<int, 2>()) : rows(std::integral_constant<int, 1>());
 }
