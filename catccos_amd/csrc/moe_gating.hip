@@ -683,7 +683,7 @@ extern "C" int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, 
         else run(lanes, integral_constant<int, lanes.value == 16 ? 32 : 16>());
     };
     // 16 lanes to a row do less work, 64 are done sooner.  Measured in a graph, 64 and 16 lanes, softmax top-8 of 256 / sigmoid in 8 groups: 1024 rows 5.3 and
-    // 6.0 / 7.0 and 9.9 us, 3072 rows 6.3 and 6.1 / 8.7 and 10.1, 4096 rows 7.1 and 6.2 / 10.9 and 10.0, on 256 CUs; of 512, 4096 rows 10.5 and 10.0 / 14.9 and 15.3, 32768
+    // 6.0 / 7.0 and 9.9 us, 4096 rows 7.1 and 6.2 / 10.9 and 10.0, on 256 CUs; of 512, 4096 rows 10.5 and 10.0 / 14.9 and 15.3, 32768
     // rows 43.6 and 28.4 / 63.5 and 43.1.
     int cus;
     if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
