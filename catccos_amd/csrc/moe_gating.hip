@@ -571,7 +571,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
         border = row_bits(__ballot(border)) != 0;
         tied = border && row_bits(__ballot(tied)) != 0;
         near |= border && row_bits(__ballot(open)) != 0;
-        near |= mend && (tied || min(a.top_k + 1, rounds) > (uint32_t)LPR);
+        near |= mend && tied;
         if (tied && !mend) {
             const float zl = scores[a.top_k].x, sl = scores[a.top_k].y, bl = bias(picks[a.top_k].x);
 #pragma unroll
@@ -592,24 +592,26 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
 #pragma unroll
                 for (int d = 1; d < LPR; d *= 2) sum += __shfl_xor(sum, d);
             }
-            const uint32_t entries = min(a.top_k + 1, rounds);
+            const uint32_t entries = mend ? min(a.top_k + 1, rounds) : 0;
             double* const values = reinterpret_cast<double*>(scores);
-            const bool takes_part = mend && lane < entries;
-            const uint2 pick = picks[takes_part ? lane : 0];
-            double v = 0.0;
-            if (takes_part) {
-                const double zr = scores[lane].x;
-                v = !a.softmax ? 1.0 / (1.0 + exp(-zr)) : (!a.bias ? zr : zr == -INFINITY ? 0.0 : exp(zr - (double)most) / sum);      // (without a bias the order of the logits)
-                v = number(v + (double)bias(pick.x));
+            uint32_t* const sorted = reinterpret_cast<uint32_t*>(scores);
+            for (uint32_t r = lane; r < entries; r += LPR) {            // (each reads the score that it overwrites)
+                const double zr = scores[r].x;
+                const double v = !a.softmax ? 1.0 / (1.0 + exp(-zr)) : (!a.bias ? zr : zr == -INFINITY ? 0.0 : exp(zr - (double)most) / sum);      // (without a bias the order of the logits)
+                values[r] = number(v + (double)bias(picks[r].x));
             }
             __builtin_amdgcn_wave_barrier();
-            if (takes_part) values[lane] = v;
+            for (uint32_t r = lane; r < entries; r += LPR) {
+                const double v = values[r];
+                const uint32_t e = picks[r].x;
+                uint32_t place = 0;
+                for (uint32_t q = 0; q < entries; ++q) place += q != r && better(values[q], picks[q].x, v, e);
+                picks[r].y = place;
+            }
             __builtin_amdgcn_wave_barrier();
-            uint32_t place = 0;
-            if (takes_part)
-                for (uint32_t r = 0; r < entries; ++r) place += r != lane && better(values[r], picks[r].x, v, pick.x);
+            for (uint32_t r = lane; r < entries; r += LPR) sorted[picks[r].y] = picks[r].x;
             __builtin_amdgcn_wave_barrier();
-            if (takes_part) picks[place] = pick;
+            for (uint32_t r = lane; r < entries; r += LPR) picks[r].x = sorted[r];
             __builtin_amdgcn_wave_barrier();
         }
         for (uint64_t left = rows; left;) {                             // every lane of the wavefront sees the same bits

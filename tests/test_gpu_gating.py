@@ -207,3 +207,22 @@ def test_groups_of_every_size_and_many_experts(tokens, experts, groups, top_grou
         z = torch.randn((tokens, experts), generator=g, device="cuda").to(dtype)
         for bias in (None, 0.1 * torch.randn(experts, generator=g, device="cuda")):
             _check(z, top_k, score, bias, groups, top_groups, group_best)
+
+
+@pytest.mark.parametrize("tokens", [40, 4000])
+@pytest.mark.parametrize("top_k", [2, 15, 16, 17, 24, 40, 64])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_pairs_that_fp32_cannot_tell_apart(tokens, top_k, score):
+    """Scores in pairs: 2^-24 of a logit inside a pair, 1/16 between pairs, in random order; chosen whole pairs, a pair in part, and with a bias that swaps
+    some; short rows that are taken whole; and rows whose scores all lie together."""
+    g = torch.Generator(device="cuda").manual_seed(top_k)
+    experts = 96
+    level = -torch.arange(experts // 2, device="cuda").repeat_interleave(2) / 16.0 - 0.5
+    z = torch.where(torch.arange(experts, device="cuda") % 2 == 1, torch.nextafter(level, torch.zeros_like(level)), level)
+    z = z[torch.rand((tokens, experts), generator=g, device="cuda").argsort(dim=1)]
+    bias = torch.where(torch.rand(experts, generator=g, device="cuda") < 0.5, 2.0 ** -26, -2.0 ** -27)
+    for b in (bias, None):
+        _check(z, top_k, score, b)
+        _check(z[:, :64], top_k, score, None if b is None else b[:64], 4, 4, 2)
+    _check(z[:, :top_k], top_k, score, bias[:top_k].contiguous())
+    _check(1e-6 * torch.randn((tokens, experts), generator=g, device="cuda"), top_k, score, bias)
