@@ -401,5 +401,5 @@ extern "C" int cmx_mxfp4_moe_ffn(const void* x, const int32_t* expert_idx, const
     // Two row tiles share a reading of the activations from LDS, if that leaves workgroups for more than half of the CUs (both matmuls, two tiles and one: 32 tokens,
     // 256 experts, k = 7168 714 us and 774; 12 tokens, 64 experts, k = 5120 195 and 203; 31 tokens, 16 experts, k = 4992 126 and 146; 20 tokens, 128
     // experts, k = 4096 158 and 124).
-    return ceil_div(k, 32) * 16 >= 9 * (uint32_t)cus ? rows(std::integral_constant<int, 2>()) : rows(std::integral_constant<int, 1>());
+    return ceil_div(k, 16) > (uint32_t)cus ? rows(std::integral_constant<int, 2>()) : rows(std::integral_constant<int, 1>());
 }
