@@ -2,12 +2,12 @@
 //
 //   t = x + residual,   r = 1 / sqrt(mean(t^2) + eps),   y = t * r * weight
 //
-// in fp32; t and y are rounded once each, to the type of x, and the codes are made of y before that rounding.  A row is read
+// in fp32; t and y are rounded once each, to the type of x, and codes and scales are those of the exact y of t (finish8).  A row is read
 // once: its elements stay in registers between the sum of squares and the scaling (a row that is too long for the registers of one
 // workgroup is read twice, the second time mostly from the caches).
 // Work split: a thread holds pieces of eight consecutive elements, so that four neighbouring lanes hold one MX block, whose
 // maximum is then two DPP exchanges away.  Short rows are a wavefront's, which needs no barrier, longer ones a workgroup's.
-// Bound by memory.  With a residual, total and codes of bf16 rows: 8192 x 7168 in 78 us (5.3 TB/s; a plain copy reaches 5.2), of 4096 columns to
+// Bound by memory.  With a residual, total and codes of bf16 rows: 8192 x 7168 in 80 us (5.2 TB/s, as a plain copy), of 4096 columns to
 // bf16 6.4 TB/s; rows of odd length, whose pieces lie across cache lines, 3.6 to 4.1.  A single row takes 3.1 us, of which 2.5 are the launch's.
 #include "mx_launch.h"
 
@@ -155,6 +155,15 @@ __device__ __forceinline__ uint32_t quantize8(const float (&y)[8], uint32_t (&w)
     }
 }
 
+// d to fp32 so that a later rounding to fewer bits, and the exponent, are those of d: towards zero, the last bit set if anything was cut off
+__device__ __forceinline__ float to_odd(double d) {
+    const float f = (float)d;
+    uint32_t bits = __float_as_uint(f);
+    if (fabs((double)f) > fabs(d)) --bits;
+    if ((double)f != d) bits |= 1u;
+    return __uint_as_float(bits);
+}
+
 struct NormArgs {
     const uint8_t* x;
     const uint8_t* residual;   // may be null
@@ -170,14 +179,39 @@ struct NormArgs {
 };
 
 // where a piece's results go; v = t, the weight beside it; every lane of a quad comes here
+// squares: the sum over the row, rstd from it in fp32
 template <int TYPE, int WTYPE>
-__device__ __forceinline__ void finish8(const NormArgs& a, size_t row, uint32_t col, const float (&v)[8], const Raw<WTYPE>& weight, float rstd) {
+__device__ __forceinline__ void finish8(const NormArgs& a, size_t row, uint32_t col, const float (&v)[8], const Raw<WTYPE>& weight, float rstd, double squares) {
     const uint32_t left = col < a.cols ? a.cols - col : 0;
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = (uint32_t)i < left ? v[i] * rstd * value<WTYPE>(weight, i) : 0.0f;
     if (a.y && left) store8<TYPE>(a.y + row * a.ld_y + (size_t)col * Elem<TYPE>::bytes, y, left);
     if (!a.codes) return;
+    // Codes and scale are to be those of the exact y.  In fp32 it is off by less than kNear units in the last place, which matters next to a border between
+    // codes or a power of two: places where the bits that no code keeps are zeros (a border's last bit is one behind a code's).  There, in one piece of
+    // 60, the wavefront computes its y again in 64 bits.  (8192 x 7168 bf16, residual: 80 us, without this 76 and 36 of 59 million codes on the wrong side.)
+    constexpr uint32_t kNear = 8;
+    const uint32_t kept = a.fmt == CMX_FMT_E4M3 ? 13 : (a.fmt == CMX_FMT_E5M2 ? 12 : 11);
+    const auto place = [&](float f) { return (__float_as_uint(f) << kept) + (kNear << kept); };
+    uint32_t nearest = ~0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nearest = min(nearest, place(y[i]));
+    if (__any(nearest <= 2 * kNear << kept)) {
+        bool near = false;                                                   // (zeros are near by their bits only)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) near |= y[i] != 0.0f && place(y[i]) <= 2 * kNear << kept;
+        if (__any(near) && rstd > 0.0f) {                                    // (0: the squares passed fp32)
+            asm volatile("" : "+v"(squares));                                // (or what this needs is computed, or held in 64 bits, by all)
+            const double exact = 1.0 / sqrt(squares / (double)a.cols + (double)a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float t = v[i];
+                asm volatile("" : "+v"(t));
+                y[i] = (uint32_t)i < left ? to_odd((double)t * exact * (double)value<WTYPE>(weight, i)) : 0.0f;
+            }
+        }
+    }
     uint32_t w[2], byte;
     if (a.fmt == CMX_FMT_E4M3) byte = quantize8<CMX_FMT_E4M3>(y, w);
     else if (a.fmt == CMX_FMT_E5M2) byte = quantize8<CMX_FMT_E5M2>(y, w);
@@ -212,13 +246,13 @@ __device__ __forceinline__ void finish8(const NormArgs& a, size_t row, uint32_t 
 
 // sum over the TPR threads of a row; every one of them gets it
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* shared) {
+__device__ __forceinline__ double row_sum(double v, double* shared) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     if constexpr (TPR > 64) {
         if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.0f;
+        v = 0.0;
 #pragma unroll
         for (int i = 0; i < TPR / 64; ++i) v += shared[i];
     }
@@ -231,7 +265,7 @@ __device__ __forceinline__ float inverse_rms(float squares, uint32_t cols, float
 template <int TYPE, int WTYPE, int TPR, int PIECES>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
     constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
-    __shared__ float shared[kThreads / 64];
+    __shared__ double shared[kThreads / 64];
     const uint32_t lane = threadIdx.x % TPR;
     const size_t row = (size_t)blockIdx.x * kRows + threadIdx.x / TPR;
     if (kRows > 1 && row >= a.rows) return;                                  // (whole wavefronts; such rows share no barrier)
@@ -257,29 +291,30 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
             load_end<WTYPE>(w[p], a.weight + (size_t)col * Elem<WTYPE>::bytes, left);
         }
     }
-    float squares = 0.0f;
+    double squares = 0.0;
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
         const uint32_t col = (lane + p * TPR) * 8, left = col < a.cols ? a.cols - col : 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             v[p][i] = value<TYPE>(x[p], i) + (a.residual ? value<TYPE>(r[p], i) : 0.0f);
-            squares += v[p][i] * v[p][i];
+            squares = fma((double)v[p][i], (double)v[p][i], squares);
         }
         if (a.total && left) store8<TYPE>(a.total + row * a.ld_total + (size_t)col * Elem<TYPE>::bytes, v[p], left);
     }
-    const float rstd = inverse_rms(row_sum<TPR>(squares, shared), a.cols, a.eps);
+    squares = row_sum<TPR>(squares, shared);
+    const float rstd = inverse_rms((float)squares, a.cols, a.eps);
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
         const uint32_t col = (lane + p * TPR) * 8;
-        if (col - (lane & 3) * 8 < a.cols) finish8<TYPE, WTYPE>(a, row, col, v[p], w[p], rstd);      // (whole quads)
+        if (col - (lane & 3) * 8 < a.cols) finish8<TYPE, WTYPE>(a, row, col, v[p], w[p], rstd, squares);      // (whole quads)
     }
 }
 
 // rows of any length: two passes
 template <int TYPE, int WTYPE>
 __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a) {
-    __shared__ float shared[16];
+    __shared__ double shared[16];
     const size_t row = blockIdx.x;
     // elements [col, col + 8) of t, zeros behind the row
     const auto piece = [&](uint32_t col, float (&v)[8]) {
@@ -295,20 +330,22 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = value<TYPE>(x, i) + (a.residual ? value<TYPE>(r, i) : 0.0f);
     };
-    float squares = 0.0f, v[8];
+    double squares = 0.0;
+    float v[8];
     for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
         piece(col, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) squares += v[i] * v[i];
+        for (int i = 0; i < 8; ++i) squares = fma((double)v[i], (double)v[i], squares);
     }
-    const float rstd = inverse_rms(row_sum<1024>(squares, shared), a.cols, a.eps);
+    squares = row_sum<1024>(squares, shared);
+    const float rstd = inverse_rms((float)squares, a.cols, a.eps);
     for (uint32_t col = threadIdx.x * 8; col - (threadIdx.x & 3) * 8 < a.cols; col += 8192) {        // (whole quads)
         piece(col, v);
         const uint8_t* const wp = a.weight + (size_t)col * Elem<WTYPE>::bytes;
         Raw<WTYPE> w = load8<WTYPE>(wp, col + 8 <= a.cols);
         if (col < a.cols && col + 8 > a.cols) load_end<WTYPE>(w, wp, a.cols - col);
         if (a.total && col < a.cols) store8<TYPE>(a.total + row * a.ld_total + (size_t)col * Elem<TYPE>::bytes, v, a.cols - col);
-        finish8<TYPE, WTYPE>(a, row, col, v, w, rstd);
+        finish8<TYPE, WTYPE>(a, row, col, v, w, rstd, squares);
     }
 }
 

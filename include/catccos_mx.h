@@ -107,7 +107,7 @@ int cmx_mx_dequant(const uint8_t* codes, uint32_t ld_codes, const uint8_t* scale
  * matmul, the gate or the experts of a layer (no counterpart in the reference, whose operators start at the activations).
  *   t = x + residual;   y = t / sqrt(mean(t^2) + eps) * weight
  * in fp32, from any input type; total receives t and y_out y, each rounded once to the type of x; codes and scales are those of
- * y before that rounding, nearest-even, by the rules and in the layout of cmx_mx_quant (padding column and non-finite blocks
+ * the exact y of t (not of its fp32 value), nearest-even, by the rules and in the layout of cmx_mx_quant (padding column and non-finite blocks
  * among them).
  *
  *   x         [rows, cols] of `type` (CMX_OUT_BF16 / FP16 / FP32), pitch ld_x elements

@@ -226,3 +226,25 @@ def test_many_rows_of_middling_length(cols, x, w, residual):
     _assert_codes(codes, scales, y, "E4M3")
     if residual:
         assert torch.equal(total, (a.float() + r.float()).to(a.dtype))
+
+
+@pytest.mark.parametrize("x,w,residual", [("bf16", "bf16", True), ("bf16", "fp32", False), ("fp16", "fp16", True), ("fp32", "fp32", True)])
+@pytest.mark.parametrize("rows,cols", [(20000, 96), (6000, 1000), (5000, 1531), (1500, 4096), (700, 12288), (300, 20007)])
+def test_codes_are_those_of_the_exact_norm(rows, cols, x, w, residual):
+    """Every code and every scale of millions, in all formats, against 64 bits with no tolerance: fp32 arithmetic would put about one in a million elsewhere."""
+    from catccos_amd import ops
+    a, r, weight = _inputs(rows, cols, x, w, residual, rows)
+    t = a.float() if r is None else a.float() + r.float()
+    y = t.double() / torch.sqrt(t.double().pow(2).mean(dim=1, keepdim=True) + float(np.float32(1e-6))) * weight.double()
+    nb = -(-cols // 32)
+    amax = torch.nn.functional.pad(y, (0, nb * 32 - cols)).view(rows, nb, 32).abs().amax(dim=2)
+    for fmt, (emax, mantissa, least, most) in FORMATS.items():
+        codes, scales, _, _ = ops.rms_norm_quant(a, weight, residual=r, fmt=fmt)
+        exp = torch.frexp(amax).exponent - 1 - emax
+        exp = torch.where(amax < 1e-12, 0, exp)
+        assert torch.equal(scales[:, :nb].int(), (exp + 127).int())
+        target = torch.ldexp(y, -exp.repeat_interleave(32, dim=1)[:, :cols])
+        step = torch.exp2((torch.frexp(target.abs().clamp_min(2.0 ** least)).exponent - 1 - mantissa).double())
+        want = (torch.round(target / step) * step).clamp(-most, most)
+        off = (_values(codes, fmt, cols) != want).sum()
+        assert int(off) == 0, (fmt, int(off))
