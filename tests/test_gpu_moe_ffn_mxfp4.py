@@ -70,6 +70,23 @@ def test_wide_rows(tokens):
     check(ops.mxfp4_moe_ffn(x, idx, gate, *w), x, idx, gate, *w)
 
 
+def test_experts_past_four_gib():
+    """W1 of 5 GB: experts on both sides of an offset of 2^32 bytes, weights and sums of the named ones against the formula."""
+    e, n, k, named = 600, 1024, 16384, [0, 255, 511, 512, 513, 599]
+    few = experts_of(len(named), n, k, 21)
+    w = [torch.zeros((e, *t.shape[1:]), dtype=torch.uint8, device="cuda") for t in few]
+    assert w[0].numel() > 1 << 32
+    for whole, part in zip(w, few):
+        whole[torch.tensor(named, device="cuda")] = part
+    x = torch.randn((3, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).to(torch.bfloat16)
+    local = torch.tensor([[0, 5], [2, 3], [4, 1]], dtype=torch.int32, device="cuda")
+    gate = torch.tensor([[0.75, 0.25], [0.5, 0.5], [1.0, 0.125]], device="cuda")
+    idx = torch.tensor(named, dtype=torch.int32, device="cuda")[local.long()].contiguous()
+    got = ops.mxfp4_moe_ffn(x, idx, gate, *w)
+    check(got, x, local, gate, *few)
+    assert torch.equal(got, ops.mxfp4_moe_ffn(x, local, gate, *few))
+
+
 def test_captured_right_after_init():
     """First launches inside a stream capture, after cmx_init() alone (tests/capture_decode_child.py)."""
     import os
