@@ -119,6 +119,12 @@ int launch(const GemvArgs& a, hipStream_t s) {
     if (columns <= 2) return launch<KIND, 1, 2>(a, s);
     if (columns <= 4) return launch<KIND, 1, 4>(a, s);
     if (columns <= 8 || kMost == 8) return launch_tiles<KIND, 8>(a, s);
+    // fp16: 8 columns come out of LDS in pieces, 16 have to be split behind it (16 rows of x, 4096 x 7168: one tile of rows and 16 columns 14.0 us, two and
+    // 8 11.9; 5120 x 8192 27.7 and 21.4; with two tiles under both, 24 rows of 4096 x 7168, 16 columns 16.7 and 8 20.6).
+    if constexpr (KIND == kXFp16) {
+        const auto two_tiles = [&](uint32_t by) { return 4 * (uint64_t)ceil_div(a.n, 32) * ceil_div(a.m, by) >= 3 * (uint64_t)cus; };
+        if (!two_tiles(16) && two_tiles(8)) return launch<KIND, 2, 8>(a, s);
+    }
     return launch_tiles<KIND, kMost>(a, s);
 }
 
