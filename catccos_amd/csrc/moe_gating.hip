@@ -24,12 +24,15 @@ namespace {
 
 constexpr uint32_t kWaves = 4, kMaxTopK = 64, kMaxGroups = 64, kMaxExperts = 1024;
 
-// How far an fp32 score as the choice computes it may be off.  Softmax, relative: exp2 of (z - max) * log2(e), whose rounding costs d = |z - max| units of 2^-24,
-// sums of up to 1024 terms (16 in a lane, then pairs), a reciprocal and two products: (d + 26) * 2^-24, below 2^-17 to d = 100; scores beyond d = 38 are off
-// by less than kTiny anyway.  Sigmoid: exp2, one addition, one reciprocal: s (1 - s) |z| + 3 s + 1 / 2 units of 2^-24, below 2^-22 for any z, and
-// (|z| + 5) * 2^-24 of a small s, below 2^-18 of it to |z| = 59.
+// How far an fp32 score as the choice computes it may be off, in units of 2^-24.  Softmax, d = max - z: the difference, the product with log2(e) and that
+// constant's own rounding cost 2.3 d of the score, exp2 2, a division and a product 2, the sum that divides 35 additions (32 in a lane, then pairs) and what its
+// terms are off, their d on average no more than ln(1024): 18.  (2.3 d + 57) s is below 2^-17 s to d = 30, what it is more from there on below kSumLoss s + kTiny;
+// and it is below 2^-18 of the row's largest score for any d.  Sigmoid: exp2, one addition, one reciprocal: s (1 - s) (1.3 |z| + 2) + 3 s, below 2^-22 for any z, and
+// (1.3 |z| + 5) s, below 2^-18 of a small s to |z| = 45, what it is more from there on below kTiny.
 constexpr float kSumLoss = 0x1p-22f, kTiny = 0x1p-70f;
 __device__ __forceinline__ float score_loss(float s, bool softmax) { return softmax ? 0x1p-17f * s : fminf(0x1p-22f, 0x1p-18f * s); }
+// of any score of a row
+__device__ __forceinline__ float widest_loss(float largest, bool softmax) { return softmax ? 0x1p-18f * largest : 0x1p-22f; }
 
 struct GateArgs {
     const uint8_t* logits;
@@ -347,16 +350,18 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
 
     bool near = false;                                                  // the row is to be done in 64 bits
     uint64_t kept = ~0ull;                                              // groups
+    // How far c may be off by its score s.  Two values that are clear of each other have to settle all that lie behind the lower one, so that the allowance must
+    // fall along the order of c: without a bias it is the score's own, with one the row's widest.
+    const float widest = widest_loss(share, a.softmax);
+    const auto choice_loss = [&](float s) { return a.bias ? widest : score_loss(s, a.softmax); };
     if (a.groups > 1) {
         float* const values = reinterpret_cast<float*>(mine + lds.group_values) + sub * a.groups;
         float* const losses = reinterpret_cast<float*>(mine + lds.losses) + sub * a.groups;
-        const float largest = a.softmax ? share : 1.0f;
         const auto enter = [&](uint32_t g, uint32_t first, uint32_t second) {
             const bool both = a.group_best == 2 && second;
             const float p = unord(first), q = both ? unord(second) : 0.0f;
             values[g] = both ? fmaxf(p + q, -INFINITY) : p;             // (not a NaN)
-            // how far the sum may be off: without a bias its own size says how large its scores are, with one the row's largest does
-            losses[g] = 2.0f * score_loss(a.bias ? largest : p + q, a.softmax) + kSumLoss * (fabsf(p) + fabsf(q));
+            losses[g] = 2.0f * choice_loss(p + q) + kSumLoss * (fabsf(p) + fabsf(q));
         };
         const uint32_t over = a.members / kChunk;                       // lanes that a group lies in
         if (kChunk == 4 && a.members % 4 == 0 && (over & (over - 1)) == 0 && over <= (uint32_t)LPR) {
@@ -553,7 +558,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
     if (!a.by_logit) {
         // closer than fp32 can tell: values c of scores s
         const auto close = [&](float c, float s, float d, float t) {
-            return !(fabsf(c - d) > score_loss(s, a.softmax) + score_loss(t, a.softmax) + kSumLoss * (fabsf(c) + fabsf(d)) + kTiny);
+            return !(fabsf(c - d) > choice_loss(s) + choice_loss(t) + kSumLoss * (fabsf(c) + fabsf(d)) + kTiny);
         };
         // Neighbours in the order: clear, of equal logits and biases (then the lower index comes first, rightly), or close.  Close ones are put in order
         // by their values in 64 bits, the first that is not chosen among them.  That is all if the second behind is clear of it; if not, more may lie there.

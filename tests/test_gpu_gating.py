@@ -226,3 +226,31 @@ def test_pairs_that_fp32_cannot_tell_apart(tokens, top_k, score):
         _check(z[:, :64], top_k, score, None if b is None else b[:64], 4, 4, 2)
     _check(z[:, :top_k], top_k, score, bias[:top_k].contiguous())
     _check(1e-6 * torch.randn((tokens, experts), generator=g, device="cuda"), top_k, score, bias)
+
+
+@pytest.mark.parametrize("tokens", [300, 4000])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_scores_of_different_size_under_cancelling_biases(tokens, score):
+    """Small scores, which fp32 knows to many places, and large ones, brought together by biases: two small ones that are clear of each other settle nothing
+    about a large one that fp32 puts behind both."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    experts = 64
+    large = torch.arange(experts, device="cuda") % 2 == 1
+    base = torch.where(large, 1 + 3 * torch.rand(experts, generator=g, device="cuda"), -7 + 2 * torch.rand(experts, generator=g, device="cuda"))
+    s = torch.softmax(base.double(), dim=0) if score == "softmax" else torch.sigmoid(base.double())
+    apart = (2 * torch.rand(experts, generator=g, device="cuda").double() - 1) * (5e-8 if score == "softmax" else 4e-7)
+    bias = ((0.0005 if score == "softmax" else 0.01) + apart - s).float()
+    step = torch.randint(-3, 4, (tokens, experts), generator=g, device="cuda", dtype=torch.int32)
+    z = (base.expand(tokens, experts).contiguous().view(torch.int32) + step).view(torch.float32)
+    for top_k in (1, 2, 5, 16, 30):
+        _check(z, top_k, score, bias)
+        _check(z, min(top_k, 8), score, bias, 4, 1, 1)
+        _check(z, top_k, score, bias, 4, 2, 2)
+
+
+def test_a_large_score_behind_two_small_ones_that_are_clear():
+    for z, bias in (([-60.0, -60.0, 2.0], [1.49e-7, 1.34e-7, 1.69e-7 - 1 / (1 + math.exp(-2.0))]), ([-7.0, -7.0, 2.4627566], [0.009088952, 0.00908894, -0.91148925])):
+        for tokens in (1, 4000):
+            row = torch.tensor(z, device="cuda").expand(tokens, 3).contiguous()
+            for top_k in (1, 2, 3):
+                _check(row, top_k, "sigmoid", torch.tensor(bias, device="cuda"))
