@@ -253,15 +253,14 @@ struct GateLds {
     static constexpr uint32_t kRows = 64 / LPR, kCapacity = LPR * SLOTS, kList = LPR == 16 ? 64 : 0;      // candidates of a row
     static constexpr uint32_t kOrdWords = kRows * kCapacity > 2 * kCapacity ? kRows * kCapacity : 2 * kCapacity;
     uint32_t list, scores, picks, ords, group_values, losses, bytes;
-    __host__ __device__ GateLds(uint32_t groups, uint32_t top_k) {
-        list = groups * 8;                                              // group values in 64 bits before it
-        scores = list + kRows * kList * 8;
-        picks = scores + kRows * (top_k + 2) * 8;
-        ords = picks + kRows * (top_k + 2) * 8;
-        group_values = ords + kOrdWords * 4;
-        losses = group_values + kRows * groups * 4;
-        bytes = (losses + kRows * groups * 4 + 7) & ~7u;
-    }
+    __host__ __device__ constexpr GateLds(uint32_t groups, uint32_t top_k)
+        : list(groups * 8),                                             // group values in 64 bits before it
+          scores(list + kRows * kList * 8),
+          picks(scores + kRows * (top_k + 2) * 8),
+          ords(picks + kRows * (top_k + 2) * 8),
+          group_values(ords + kOrdWords * 4),
+          losses(group_values + kRows * groups * 4),
+          bytes((losses + kRows * groups * 4 + 7) & ~7u) {}
 };
 
 // LPR lanes per row, SLOTS experts per lane
@@ -674,28 +673,32 @@ extern "C" int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, 
                         experts / groups, top_groups, group_best, ceil_div(1u << 20, experts / groups), scale, type, score == CMX_SCORE_SOFTMAX, renormalize != 0,
                         !bias && (groups == 1 || group_best == 1 || experts == groups)};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const auto run = [&](auto lanes, auto slots) {
+    const auto run = [&](auto lanes, auto slots) -> int {
         const GateLds<lanes.value, slots.value> lds(groups, top_k);
+        constexpr size_t kMostLds = kWaves * GateLds<lanes.value, slots.value>(kMaxGroups, kMaxTopK).bytes;
+        if constexpr (kMostLds > 64 * 1024) {                           // (512 experts, 64 groups and top_k 64 by 16 lanes: 66.5 KiB)
+            if (int rc = allow_dynamic_lds<moe_gating_kernel<lanes.value, slots.value>, kMostLds>(); rc != CMX_OK) return rc;
+        }
         hipLaunchKernelGGL((moe_gating_kernel<lanes.value, slots.value>), dim3(ceil_div(tokens, 64 / lanes.value * kWaves)), dim3(64 * kWaves),
                            kWaves * lds.bytes, s, a);
+        CMX_LAUNCH_CHECK();
+        return CMX_OK;
     };
     using std::integral_constant;
-    const auto by_slots = [&](auto lanes) {
+    const auto by_slots = [&](auto lanes) -> int {
         const uint32_t slots = ceil_div(experts, lanes.value);
-        if (slots <= 1) run(lanes, integral_constant<int, 1>());
-        else if (slots <= 2) run(lanes, integral_constant<int, 2>());
-        else if (slots <= 4) run(lanes, integral_constant<int, 4>());
-        else if (slots <= 8) run(lanes, integral_constant<int, 8>());
-        else if (slots <= 16 || lanes.value == 64) run(lanes, integral_constant<int, 16>());
-        else run(lanes, integral_constant<int, lanes.value == 16 ? 32 : 16>());
+        if (slots <= 1) return run(lanes, integral_constant<int, 1>());
+        if (slots <= 2) return run(lanes, integral_constant<int, 2>());
+        if (slots <= 4) return run(lanes, integral_constant<int, 4>());
+        if (slots <= 8) return run(lanes, integral_constant<int, 8>());
+        if (slots <= 16 || lanes.value == 64) return run(lanes, integral_constant<int, 16>());
+        return run(lanes, integral_constant<int, lanes.value == 16 ? 32 : 16>());
     };
     // 16 lanes to a row do less work, 64 are done sooner.  Measured in a graph, 64 and 16 lanes, softmax top-8 of 256 / sigmoid in 8 groups: 1024 rows 5.3 and
     // 6.0 / 7.0 and 9.9 us, 4096 rows 7.1 and 6.2 / 10.9 and 10.0, on 256 CUs; of 512, 4096 rows 10.5 and 10.0 / 14.9 and 15.3, 32768
     // rows 43.6 and 28.4 / 63.5 and 43.1.
     int cus;
     if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
-    if (tokens >= 14u * (uint32_t)cus && experts <= 512) by_slots(integral_constant<int, 16>());
-    else by_slots(integral_constant<int, 64>());
-    CMX_LAUNCH_CHECK();
-    return CMX_OK;
+    if (tokens >= 14u * (uint32_t)cus && experts <= 512) return by_slots(integral_constant<int, 16>());
+    return by_slots(integral_constant<int, 64>());
 }

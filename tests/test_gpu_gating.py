@@ -254,3 +254,24 @@ def test_a_large_score_behind_two_small_ones_that_are_clear():
             row = torch.tensor(z, device="cuda").expand(tokens, 3).contiguous()
             for top_k in (1, 2, 3):
                 _check(row, top_k, "sigmoid", torch.tensor(bias, device="cuda"))
+
+
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [(512, 64, 64, 64), (320, 64, 40, 64), (384, 64, 13, 58), (520, 52, 30, 64), (512, 64, 8, 64)])
+def test_the_most_groups_and_the_largest_top_k_of_many_rows(experts, groups, top_groups, top_k):
+    """Workgroups that hold more than 64 KiB of lists: up to 512 experts, 14 rows and more to a CU."""
+    tokens = 14 * torch.cuda.get_device_properties(0).multi_processor_count + 5
+    z, bias = _logits(tokens, experts, "fp32", experts)
+    for score in ("softmax", "sigmoid"):
+        for b in (None, bias):
+            _check(z, top_k, score, b, groups, top_groups, 2)
+    _check(z.half(), top_k, "sigmoid", bias, groups, top_groups, 1)
+
+
+def test_the_largest_workgroups_captured_right_after_init():
+    """Their first launch inside a stream capture, after cmx_init() alone (tests/capture_gating_child.py)."""
+    import os
+    import subprocess
+    import sys
+    child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "capture_gating_child.py")
+    r = subprocess.run([sys.executable, child], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "CAPTURE-OK" in r.stdout, (r.returncode, r.stdout[-2000:], r.stderr[-2000:])
