@@ -310,7 +310,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
         }
     }
 
-    bool poisoned = false;                                              // softmax: a NaN or +Inf makes every score NaN
+    bool poisoned = false;                                              // softmax: a NaN or +Inf makes every score NaN, and the lowest indices are chosen
     float most = -INFINITY, total = 0.0f;
     if (a.softmax) {
 #pragma unroll
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
         // groups that fp32 cannot tell from one on the other side of the border: their values in 64 bits decide
         lowest = -row_max<LPR>(-lowest);
         highest = row_max<LPR>(highest);
-        near = !a.by_logit && a.top_groups < a.groups && !(lowest > highest + kTiny);
+        near = !a.by_logit && !poisoned && a.top_groups < a.groups && !(lowest > highest + kTiny);
         if (near && a.groups <= (uint32_t)LPR) {
             near = false;
             if (lane < a.groups) near = kept >> lane & 1ull ? !(values[lane] - losses[lane] > highest + kTiny) : !(values[lane] + losses[lane] < lowest - kTiny);
@@ -571,8 +571,8 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
             tied |= same && r == a.top_k;
             open |= unclear && r == a.top_k;
         }
-        mend = row_bits(__ballot(mend)) != 0;
-        border = row_bits(__ballot(border)) != 0;
+        mend = !poisoned && row_bits(__ballot(mend)) != 0;
+        border = !poisoned && row_bits(__ballot(border)) != 0;
         tied = border && row_bits(__ballot(tied)) != 0;
         near |= border && row_bits(__ballot(open)) != 0;
         near |= mend && tied;

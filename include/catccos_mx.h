@@ -345,8 +345,8 @@ int cmx_int8_gmm_dequant_swiglu(const int8_t* a, uint32_t lda, const float* toke
  *   scale_bits   scale as the 32 bits of a float
  *   expert_idx   int32 [tokens, top_k], gate_weight fp32 [tokens, top_k]
  * tokens < 2^26, experts <= 1024, groups <= 64 and a divisor of experts, top_k <= 64.  A logit or bias of -Inf masks an expert: it is chosen
- * when no other is left.  A row of -Inf has scores of zero.  NaN is chosen like -Inf; a NaN or +Inf in a softmax row makes
- * its weights NaN.  Whatever a row holds, its indices are distinct and in [0, experts).
+ * when no other is left.  A row of -Inf has scores of zero.  NaN is chosen like -Inf.  A NaN or +Inf in a softmax row makes
+ * its scores and weights NaN: where scores are compared, not logits, the lowest indices are chosen.  Whatever a row holds, its indices are distinct and in [0, experts).
  * ---------------------------------------------------------------------------------------- */
 int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, const float* bias, uint32_t tokens, uint32_t experts,
                    uint32_t top_k, int score, uint32_t groups, uint32_t top_groups, uint32_t group_best, int renormalize,

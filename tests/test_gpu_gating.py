@@ -275,3 +275,22 @@ def test_the_largest_workgroups_captured_right_after_init():
     child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "capture_gating_child.py")
     r = subprocess.run([sys.executable, child], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "CAPTURE-OK" in r.stdout, (r.returncode, r.stdout[-2000:], r.stderr[-2000:])
+
+
+@pytest.mark.parametrize("tokens", [41, 4001])
+def test_softmax_rows_that_hold_a_nan_or_inf_have_no_order(tokens):
+    """Every score is NaN, which counts as -Inf: the lowest indices, whatever else the row holds, where scores are compared; the rows beside are not touched."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    z = torch.randn((tokens, 96), generator=g, device="cuda")
+    z = torch.where(torch.rand(z.shape, generator=g, device="cuda") < 0.5, -math.inf, z)
+    poisoned = torch.arange(tokens, device="cuda") % 3 != 0
+    z[poisoned, 70] = torch.where(torch.arange(tokens, device="cuda") % 2 == 0, math.nan, math.inf)[poisoned]
+    bias = 0.5 + 0.1 * torch.randn(96, generator=g, device="cuda")
+    for b, args in ((bias, (1, 1, 1)), (bias, (8, 4, 2)), (bias, (8, 3, 1)), (bias, (48, 20, 2)), (None, (8, 4, 2)), (None, (48, 20, 2))):
+        for top_k in (1, 5, 20, 36):
+            idx, w = ops.moe_gating(z, top_k, "softmax", b, *args)
+            assert bool((idx[poisoned] == torch.arange(top_k, device="cuda")).all()), (args, top_k)
+            assert bool(w[poisoned].isnan().all())
+            _check(z[~poisoned], top_k, "softmax", b, *args)
+            want = ops.moe_gating(z[~poisoned], top_k, "softmax", b, *args)
+            assert torch.equal(idx[~poisoned], want[0])
