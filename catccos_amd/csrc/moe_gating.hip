@@ -222,6 +222,10 @@ __device__ __forceinline__ void choose_exactly(const GateArgs& a, const uint8_t*
             for (uint32_t g = 0; g < a.groups; ++g) rank += g != lane && better(group_value[g], g, group_value[lane], lane);
         kept = __ballot(lane < a.groups && rank < a.top_groups);
     }
+    if (!a.bias) {                                                      // the order of the logits, also where 64 bits round their scores to one or to zero
+        for (uint32_t e = lane; e < a.experts; e += 64) value[e] = number((double)logit(a, row, e));
+        __builtin_amdgcn_wave_barrier();
+    }
     uint32_t taken = 0;                                                 // of this lane's experts lane, lane + 64, ...
     for (uint32_t r = 0; r < a.top_k; ++r) {
         double best = 0.0;
@@ -601,7 +605,7 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
             uint32_t* const sorted = reinterpret_cast<uint32_t*>(scores);
             for (uint32_t r = lane; r < entries; r += LPR) {            // (each reads the score that it overwrites)
                 const double zr = scores[r].x;
-                const double v = !a.softmax ? 1.0 / (1.0 + exp(-zr)) : (!a.bias ? zr : zr == -INFINITY ? 0.0 : exp(zr - (double)most) / sum);      // (without a bias the order of the logits)
+                const double v = !a.bias ? zr : (!a.softmax ? 1.0 / (1.0 + exp(-zr)) : zr == -INFINITY ? 0.0 : exp(zr - (double)most) / sum);      // (without a bias the order of the logits)
                 values[r] = number(v + (double)bias(picks[r].x));
             }
             __builtin_amdgcn_wave_barrier();

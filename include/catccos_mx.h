@@ -337,8 +337,8 @@ int cmx_int8_gmm_dequant_swiglu(const int8_t* a, uint32_t lda, const float* toke
  *   kept groups: the top_groups of `groups` groups of experts / groups neighbours whose group_best (1 or 2) largest c have the
  *   largest sum;  chosen: the top_k largest c in them, in falling order;  gate_weight = s * scale, with renormalize over
  *   the sum of the chosen s first (zero if that is zero).  Ties go to the lower index, for groups too.
- * The order is that of the exact values, not of values rounded to fp32: without a bias and with one value for each group logits are compared, elsewhere
- * c in up to 64 bits.
+ * The order is that of the exact values, not of values rounded to fp32: without a bias experts are compared by their logits, with one by c in up to 64 bits;
+ * groups by logits where one value of a group is asked for and there is no bias, elsewhere by sums in up to 64 bits.
  *
  *   logits       [tokens, experts] of `type` (CMX_OUT_BF16 / FP16 / FP32), pitch ld_logits elements
  *   bias         fp32 [experts] or NULL; it moves the choice, not the weights

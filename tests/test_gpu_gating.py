@@ -294,3 +294,29 @@ def test_softmax_rows_that_hold_a_nan_or_inf_have_no_order(tokens):
             _check(z[~poisoned], top_k, "softmax", b, *args)
             want = ops.moe_gating(z[~poisoned], top_k, "softmax", b, *args)
             assert torch.equal(idx[~poisoned], want[0])
+
+
+@pytest.mark.parametrize("tokens", [37, 4003])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_without_a_bias_the_order_is_the_logits_where_scores_are_lost(tokens, score):
+    """Logits whose scores even 64 bits round to one or to zero, in groups that are compared by sums of two scores: the kept groups' experts come in the order
+    of their logits, and masked ones behind all others."""
+    g = torch.Generator(device="cuda").manual_seed(41)
+    z = torch.randn((tokens, 64), generator=g, device="cuda")
+    z = torch.where(torch.rand(z.shape, generator=g, device="cuda") < 0.3, -math.inf, z * 30 - 2000)      # scores of zero
+    if score == "sigmoid":
+        z[:, 5::9] = 60 + 10 * torch.rand((tokens, len(range(5, 64, 9))), generator=g, device="cuda")     # and of one
+    else:
+        z[:, 9] = 1.0
+    for top_k in (1, 6, 14, 32):
+        for kept in (8, 4):
+            part = z
+            if kept == 4:                                              # groups 1, 3, 5 and 7 stand out
+                part = z.clone()
+                for n in (1, 3, 5, 7):
+                    part[:, 8 * n + 2], part[:, 8 * n + 3] = 3.0 + n, 2.0 + n
+            idx, _ = ops.moe_gating(part, top_k, score, None, 8, kept, 2)
+            key = torch.where(part == -math.inf, -1e30, part)          # masked ones last, but in front of those of closed groups
+            if kept == 4:
+                key = torch.where(torch.arange(64, device="cuda") // 8 % 2 == 1, key, -math.inf)
+            assert torch.equal(idx.long(), key.sort(dim=1, descending=True, stable=True).indices[:, :top_k]), (top_k, kept)
