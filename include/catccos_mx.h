@@ -344,8 +344,9 @@ int cmx_int8_gmm_dequant_swiglu(const int8_t* a, uint32_t lda, const float* toke
  *   bias         fp32 [experts] or NULL; it moves the choice, not the weights
  *   scale_bits   scale as the 32 bits of a float
  *   expert_idx   int32 [tokens, top_k], gate_weight fp32 [tokens, top_k]
- * tokens < 2^26, experts <= 1024, groups <= 64 and a divisor of experts, top_k <= 64.  A logit or bias of -Inf masks an expert: it is chosen
- * when no other is left.  A row of -Inf has scores of zero.  NaN is chosen like -Inf.  A NaN or +Inf in a softmax row makes
+ * tokens < 2^26, experts <= 1024, groups <= 64 and a divisor of experts, top_k <= 64.  A bias of -Inf masks an
+ * expert: it is chosen when no other is left in the kept groups.  A logit of -Inf is a score of zero: behind all others without a bias, but with one c is
+ * the bias alone, which may lie above others.  A row of -Inf has scores of zero.  NaN is chosen like -Inf.  A NaN or +Inf in a softmax row makes
  * its scores and weights NaN: where scores are compared, not logits, the lowest indices are chosen.  Whatever a row holds, its indices are distinct and in [0, experts).
  * ---------------------------------------------------------------------------------------- */
 int cmx_moe_gating(const void* logits, uint32_t ld_logits, int type, const float* bias, uint32_t tokens, uint32_t experts,

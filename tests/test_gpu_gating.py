@@ -320,3 +320,20 @@ def test_without_a_bias_the_order_is_the_logits_where_scores_are_lost(tokens, sc
             if kept == 4:
                 key = torch.where(torch.arange(64, device="cuda") // 8 % 2 == 1, key, -math.inf)
             assert torch.equal(idx.long(), key.sort(dim=1, descending=True, stable=True).indices[:, :top_k]), (top_k, kept)
+
+
+@pytest.mark.parametrize("tokens", [3, 4001])
+def test_a_logit_of_minus_inf_is_a_score_of_zero_and_a_bias_of_minus_inf_a_mask(tokens):
+    z, _ = _logits(tokens, 64, "fp32", 51)
+    masked = torch.arange(64, device="cuda") % 2 == 0
+    for score in ("softmax", "sigmoid"):
+        for args in ((1, 1, 1), (8, 8, 2), (8, 6, 1)):
+            # -Inf in the logits: behind all others without a bias; with one, c is the bias
+            away = torch.where(masked, -math.inf, z)
+            idx, w = ops.moe_gating(away, 24, score, None, *args)
+            assert not bool(masked[idx.long()].any()) and bool((w > 0).all())
+            idx, w = ops.moe_gating(away, 24, score, torch.where(masked, 2.0, 0.0), *args)
+            assert bool(masked[idx.long()].all()) and bool((w == 0).all())
+            # in the bias: behind all others, whatever the logits
+            idx, w = ops.moe_gating(torch.where(masked, z + 20, z), 24, score, torch.where(masked, -math.inf, 0.1), *args)
+            assert not bool(masked[idx.long()].any()) and bool((w > 0).all())
