@@ -129,7 +129,11 @@ __device__ __forceinline__ double row_max_key(double v) {
     return v;
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+__device__ __forceinline__ float sigmoid(float z) {
+    const bool small = z < -80.0f;                                      // (exp(-z) may overflow where the score does not)
+    const float e = expf(small ? z : -z);
+    return small ? e : 1.0f / (1.0f + e);
+}
 // what the choice makes do with (score_loss)
 __device__ __forceinline__ float quick_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 __device__ __forceinline__ float quick_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + quick_exp(-z)); }
@@ -635,6 +639,19 @@ __global__ __launch_bounds__(64 * kWaves) void moe_gating_kernel(const GateArgs 
     if (a.renormalize) {
         for (uint32_t r = lane; r < a.top_k; r += LPR) sum += scores[r].y;
         sum = row_sum<LPR>(sum);
+        // Scores that fp32 holds in part or not at all: their quotients are those of exp(z), under the largest chosen logit.  (Below 2^-23 the 1 of a sigmoid's
+        // denominator is all of it.  What 64 bits do not hold either, below exp(-745), stays zero.)
+        const bool faint = sum < 0x1p-23f;
+        if (__builtin_expect(__ballot(faint) != 0, 0)) {
+            float high = -INFINITY;
+            for (uint32_t r = lane; r < a.top_k; r += LPR) high = fmaxf(high, scores[r].x);
+            high = row_max<LPR>(high);
+            if (faint && high - (a.softmax ? most : 0.0f) > -745.0f)
+                for (uint32_t r = lane; r < a.top_k; r += LPR) scores[r].y = expf(scores[r].x - high);
+            float again = 0.0f;
+            for (uint32_t r = lane; r < a.top_k; r += LPR) again += scores[r].y;
+            sum = row_sum<LPR>(again);
+        }
     }
     for (uint32_t r = lane; r < a.top_k && live; r += LPR) {
         const float s = scores[r].y;

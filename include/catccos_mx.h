@@ -336,7 +336,7 @@ int cmx_int8_gmm_dequant_swiglu(const int8_t* a, uint32_t lda, const float* toke
  *   s = softmax(logits) or sigmoid(logits) by `score`;  c = s + bias
  *   kept groups: the top_groups of `groups` groups of experts / groups neighbours whose group_best (1 or 2) largest c have the
  *   largest sum;  chosen: the top_k largest c in them, in falling order;  gate_weight = s * scale, with renormalize over
- *   the sum of the chosen s first (zero if that is zero).  Ties go to the lower index, for groups too.
+ *   the sum of the chosen s first (zero if that is zero, or less than 64 bits hold: below exp(-745)).  Ties go to the lower index, for groups too.
  * The order is that of the exact values, not of values rounded to fp32: without a bias experts are compared by their logits, with one by c in up to 64 bits;
  * groups by logits where one value of a group is asked for and there is no bias, elsewhere by sums in up to 64 bits.
  *

@@ -337,3 +337,28 @@ def test_a_logit_of_minus_inf_is_a_score_of_zero_and_a_bias_of_minus_inf_a_mask(
             # in the bias: behind all others, whatever the logits
             idx, w = ops.moe_gating(torch.where(masked, z + 20, z), 24, score, torch.where(masked, -math.inf, 0.1), *args)
             assert not bool(masked[idx.long()].any()) and bool((w > 0).all())
+
+
+@pytest.mark.parametrize("tokens", [5, 4001])
+def test_weights_of_scores_that_fp32_cannot_hold(tokens):
+    """Chosen scores below what fp32 holds: their quotients are not.  A weight is then a quotient of exponentials of differences between chosen logits, below
+    10 here, and of their sum: fewer roundings than WEIGHT_LOSS counts."""
+    g = torch.Generator(device="cuda").manual_seed(61)
+    z = torch.randn((tokens, 64), generator=g, device="cuda")
+    low = torch.where(torch.arange(64, device="cuda") % 4 == 0, 0.0, -math.inf)           # the bias keeps these 16 out of 64
+    zero = torch.zeros(64, device="cuda")
+    for shift in (30.0, 80.0, 95.0, 110.0, 400.0, 700.0):
+        _check(z - shift, 8, "sigmoid", None)
+        _check(z - shift, 8, "sigmoid", zero, 8, 4, 2)
+        _check(z - shift, 16, "sigmoid", low, scale=2.5)
+        far = torch.where(low == 0, z - shift, z)
+        for args in ((1, 1, 1), (4, 4, 2)):
+            _check(far, 16, "softmax", low, *args)
+    # all alike: 1 / 8 each
+    w = ops.moe_gating(torch.full((tokens, 64), -95.0, device="cuda"), 8, "sigmoid")[1]
+    assert bool(((w - 0.125).abs() <= 2.0 ** -24).all())
+    # not renormalised: the score itself, rounded where fp32 has fewer bits for it
+    z = -80 - 20 * torch.rand((tokens, 64), generator=g, device="cuda")
+    idx, w = ops.moe_gating(z, 8, "sigmoid", renormalize=False)
+    want = torch.sigmoid(z.double()).gather(1, idx.long())
+    assert bool(((w.double() - want).abs() <= want * WEIGHT_LOSS + 2.0 ** -148).all())
