@@ -181,7 +181,7 @@ struct NormArgs {
 // where a piece's results go; v = t, the weight beside it; every lane of a quad comes here
 // squares: the sum over the row, rstd from it in fp32
 template <int TYPE, int WTYPE>
-__device__ __forceinline__ void finish8(const NormArgs& a, size_t row, uint32_t col, const float (&v)[8], const Raw<WTYPE>& weight, float rstd, double squares) {
+__device__ __forceinline__ void finish8(const NormArgs& a, size_t row, uint32_t col, const float (&v)[8], const Raw<WTYPE>& weight, float rstd, double squares, float eps) {
     const uint32_t left = col < a.cols ? a.cols - col : 0;
     float y[8];
 #pragma unroll
@@ -203,7 +203,7 @@ __device__ __forceinline__ void finish8(const NormArgs& a, size_t row, uint32_t 
         for (int i = 0; i < 8; ++i) near |= y[i] != 0.0f && place(y[i]) <= 2 * kNear << kept;
         if (__any(near) && rstd > 0.0f) {                                    // (0: the squares passed fp32)
             asm volatile("" : "+v"(squares));                                // (or what this needs is computed, or held in 64 bits, by all)
-            const double exact = 1.0 / sqrt(squares / (double)a.cols + (double)a.eps);
+            const double exact = 1.0 / sqrt(squares / (double)a.cols + (double)eps);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float t = v[i];
@@ -261,6 +261,11 @@ __device__ __forceinline__ double row_sum(double v, double* shared) {
 
 __device__ __forceinline__ float inverse_rms(float squares, uint32_t cols, float eps) { return 1.0f / sqrtf(squares / (float)cols + eps); }
 
+// Rows whose squares fp32 holds in part or not at all, beside an eps that is as small or zero: t is lifted by a power of two, squares and eps by its square, which
+// leaves y as it is.  From the smallest t on (2^-149) the mean of up to 2^30 squares is then a normal number, and none is too large.
+constexpr float kLift = 0x1p104f;
+__device__ __forceinline__ bool needs_lift(double squares, float eps) { return squares < 0x1p-90 && eps < 0x1p-90f; }
+
 // TPR threads per row, PIECES pieces of eight elements per thread: rows of up to 8 * TPR * PIECES elements
 template <int TYPE, int WTYPE, int TPR, int PIECES>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
@@ -303,11 +308,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
         if (a.total && left) store8<TYPE>(a.total + row * a.ld_total + (size_t)col * Elem<TYPE>::bytes, v[p], left);
     }
     squares = row_sum<TPR>(squares, shared);
-    const float rstd = inverse_rms((float)squares, a.cols, a.eps);
+    float eps = a.eps;
+    if (needs_lift(squares, eps)) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[p][i] *= kLift;
+        }
+        squares *= (double)kLift * kLift;
+        eps = eps * kLift * kLift;
+    }
+    const float rstd = inverse_rms((float)squares, a.cols, eps);
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
         const uint32_t col = (lane + p * TPR) * 8;
-        if (col - (lane & 3) * 8 < a.cols) finish8<TYPE, WTYPE>(a, row, col, v[p], w[p], rstd, squares);      // (whole quads)
+        if (col - (lane & 3) * 8 < a.cols) finish8<TYPE, WTYPE>(a, row, col, v[p], w[p], rstd, squares, eps);      // (whole quads)
     }
 }
 
@@ -338,14 +353,24 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a) {
         for (int i = 0; i < 8; ++i) squares = fma((double)v[i], (double)v[i], squares);
     }
     squares = row_sum<1024>(squares, shared);
-    const float rstd = inverse_rms((float)squares, a.cols, a.eps);
+    float eps = a.eps;
+    const bool lift = needs_lift(squares, eps);
+    if (lift) {
+        squares *= (double)kLift * kLift;
+        eps = eps * kLift * kLift;
+    }
+    const float rstd = inverse_rms((float)squares, a.cols, eps);
     for (uint32_t col = threadIdx.x * 8; col - (threadIdx.x & 3) * 8 < a.cols; col += 8192) {        // (whole quads)
         piece(col, v);
         const uint8_t* const wp = a.weight + (size_t)col * Elem<WTYPE>::bytes;
         Raw<WTYPE> w = load8<WTYPE>(wp, col + 8 <= a.cols);
         if (col < a.cols && col + 8 > a.cols) load_end<WTYPE>(w, wp, a.cols - col);
         if (a.total && col < a.cols) store8<TYPE>(a.total + row * a.ld_total + (size_t)col * Elem<TYPE>::bytes, v, a.cols - col);
-        finish8<TYPE, WTYPE>(a, row, col, v, w, rstd, squares);
+        if (lift) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= kLift;
+        }
+        finish8<TYPE, WTYPE>(a, row, col, v, w, rstd, squares, eps);
     }
 }
 

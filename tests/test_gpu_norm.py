@@ -248,3 +248,25 @@ def test_codes_are_those_of_the_exact_norm(rows, cols, x, w, residual):
         want = (torch.round(target / step) * step).clamp(-most, most)
         off = (_values(codes, fmt, cols) != want).sum()
         assert int(off) == 0, (fmt, int(off))
+
+
+@pytest.mark.parametrize("x,w", [("bf16", "bf16"), ("fp32", "fp32"), ("bf16", "fp32")])
+@pytest.mark.parametrize("cols", [96, 1000, 2048, 4100, 12288, 20007])
+@pytest.mark.parametrize("eps", [0.0, 1e-44, 1e-38])
+def test_rows_whose_squares_fp32_cannot_hold(cols, x, w, eps):
+    """Rows of 2^-20 down to the smallest numbers of the type, with an eps of their size or none: y, codes and scales are as exact as elsewhere."""
+    from catccos_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    scale = 2.0 ** -torch.tensor([20.0, 44, 46, 60, 63, 64, 70, 74, 75, 90, 110, 126, 128, 131], dtype=torch.float64, device="cuda")
+    a, r = ((torch.randn((len(scale), cols), generator=g, device="cuda").double() * scale[:, None]).to(DTYPES[x]) for _ in range(2))
+    weight = (1 + 0.3 * torch.randn(cols, generator=g, device="cuda")).to(DTYPES[w])
+    for residual in (None, r):
+        t, y = _definition(a, residual, weight, float(np.float32(eps)))
+        got_y, got_t = ops.rms_norm(a, weight, eps, residual=residual)
+        _assert_rounded(got_y, y, "y")
+        if residual is not None:
+            _assert_rounded(got_t, t, "t")
+        for fmt in FORMATS:
+            codes, scales, y2, t2 = ops.rms_norm_quant(a, weight, eps, residual=residual, fmt=fmt, want_y=True)
+            _assert_codes(codes, scales, y, fmt)
+            assert torch.equal(y2, got_y) and (residual is None or torch.equal(t2, got_t))
