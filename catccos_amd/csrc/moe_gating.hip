@@ -9,12 +9,13 @@
 //     as it is; scores are computed for the chosen experts alone (softmax, not renormalised: the sum over all in addition);
 //   - otherwise c is compared in fp32, and values that lie closer than fp32 can tell apart (score_loss), other than by equal logits and biases, are
 //     compared again in 64 bits: the groups next to the border between kept and not, the chosen and the first behind them, and the whole row where
-//     that may not be all.  With N(0, 1) logits and sigmoids one row in two thousand has such a pair.
+//     that may not be all.  With N(0, 1) logits and sigmoids one row in two thousand has such a pair; softmax with a bias has more of them where a few scores
+//     are large (8192 rows of 256: 13 us, of 3 x N(0, 1) logits 20).
 // Work split: LPR lanes hold a row, so that a wavefront works on 64 / LPR rows at a time; an expert is one key of 64 bits that
 // carries value and index.  With 16 lanes to a row the few experts that can be chosen at all are put in a list and count each other; with 64 a round
 // of the choice is one maximum over the lanes' own best keys.
-// Bound by the vector ALU where there are many rows: about 1300 instructions for four rows of 256 in 8 groups.  32768 such rows take 27 us (their 17 MB
-// would take 3), 8192 rows of fp32 logits without groups 6.2, one row 5.0, of which a launch is 2.5.
+// Bound by the vector ALU where there are many rows: 1270 instructions for four rows of 256 in 8 groups, which keep it busy for 78 % of the time.  32768 such
+// rows take 27 us (their 17 MB would take 3), 8192 rows of fp32 logits without groups 6.2, one row 5.1, of which a launch is 2.5.
 #include <type_traits>
 
 #include "mx_launch.h"

@@ -9,7 +9,7 @@
 // is taken in an order that depends on the routing alone.
 //
 // Bound by the weights of the experts that are named.  Measured, k = 7168, n = 4096, 8 of 256 experts a token: one token 24 + 16 us (187 MB, 4.6 TB/s), 32
-// tokens 445 + 300 us (3.8 GB, 5.1 TB/s).
+// tokens 715 to 740 us (3.8 GB, 5.2 TB/s), of which the first takes 445.
 #include "mx_launch.h"
 #include "mxfp4_rows.h"
 

@@ -7,8 +7,8 @@
 // workgroup is read twice, the second time mostly from the caches).
 // Work split: a thread holds pieces of eight consecutive elements, so that four neighbouring lanes hold one MX block, whose
 // maximum is then two DPP exchanges away.  Short rows are a wavefront's, which needs no barrier, longer ones a workgroup's.
-// Bound by memory.  With a residual, total and codes of bf16 rows: 8192 x 7168 in 80 us (5.2 TB/s, as a plain copy), of 4096 columns to
-// bf16 6.4 TB/s; rows of odd length, whose pieces lie across cache lines, 3.6 to 4.1.  A single row takes 3.1 us, of which 2.5 are the launch's.
+// Bound by memory.  bf16 rows with a residual and total: 8192 x 7168 to E4M3 codes in 80 us (5.2 TB/s, as a plain copy; E2M1 76), to bf16 in 83 (5.6 TB/s), of
+// 4096 columns to bf16 5.6 to 5.9 TB/s; rows of odd length, whose pieces lie across cache lines, 3.5 to 4.3.  A single row takes 3.2 us, of which 2.5 are the launch's.
 #include "mx_launch.h"
 
 namespace cmx {

@@ -194,8 +194,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual=
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual=None, fmt: str = "E4M3", want_y: bool = False, total=None):
-    """rms_norm straight to MX codes, E4M3, E5M2 or E2M1 to nearest-even: (codes, scales, y|None, t|None), codes and scales as mx_quant gives them but
-    made of the exact y."""
+    """rms_norm straight to MX codes, E4M3, E5M2 or E2M1: (codes, scales, y|None, t|None), codes and scales as mx_quant gives them by "rne" (which is not its
+    default for E2M1) but made of the exact y."""
     rows, cols = x.shape
     code_cols, s_cols = (cols + 1) // 2 if fmt in _FP4 else cols, scale_cols(cols)
     made = _norm(x, weight, eps, residual, total, (x.dtype, rows, cols) if want_y else None, (torch.uint8, rows, code_cols), (torch.uint8, rows, s_cols),

@@ -153,7 +153,8 @@ int cmx_mx_gemm(const uint8_t* a, uint32_t lda, const uint8_t* a_scale, uint32_t
  *   b        E2M1 codes [n, k/2], even column in the low nibble, pitch ld_b bytes; rows 16-byte aligned
  *   b_scale  E8M0 [n, >= k/32], pitch ld_bs bytes (as the quantizer writes it for a weight)
  *   out      [m, n] of out_type, pitch ld_out elements
- * Products are exact (fp16 and fp32 activations are split into bf16 pieces that add up to them) and sums are fp32.  k a multiple of 32.
+ * Products are exact (fp16 and fp32 activations are split into bf16 pieces that add up to them, but for what of an fp32 value lies below 2^-133) and sums
+ * are fp32.  A scale of 255 is NaN; weights past fp32 (scale bytes 253 and 254 under the larger codes) are Inf.  k a multiple of 32.
  * ---------------------------------------------------------------------------------------- */
 int cmx_mxfp4_gemv(const void* x, uint32_t ld_x, int x_type, const uint8_t* b, uint32_t ld_b, const uint8_t* b_scale,
                    uint32_t ld_bs, void* out, uint32_t ld_out, int out_type, uint32_t m, uint32_t n, uint32_t k,
