@@ -70,6 +70,12 @@ SIGNATURES = {
     "cmx_moe_token_unpermute": (i32, [vp, u32, u32, i32p, f32p, vp, u32, u32, u32, u32, vp]),
     "cmx_mxfp4_moe_ffn_workspace_bytes": (sz, [u32, u32, u32]),
     "cmx_mxfp4_moe_ffn": (i32, [vp, i32p, f32p, u8p, u8p, u8p, u8p, vp, u8p, u32, u32, u32, u32, u32, vp]),
+    "cmx_fp8_block_quant": (i32, [vp, u32, u64, i32, u8p, u32, f32p, u32, u32, u32, u32, i32, i32, i32, i32, vp]),
+    "cmx_fp8_block_gemm": (i32, [u8p, u32, f32p, u32, u8p, u32, f32p, u32, u32, vp, u32, u32, u32, u32, i32, i32, vp]),
+    "cmx_fp8_block_gmm": (i32, [u8p, u32, f32p, u32, u8p, f32p, vp, u32, i32p, u32, u32, u32, u32, i32, i32, i32, vp]),
+    "cmx_moe_token_permute": (i32, [vp, u32, i32p, vp, u32, u32, u32, u32, u32, u32, i32, vp]),
+    "cmx_moe_token_permute_grad": (i32, [vp, u32, u32, i32p, vp, u32, u32, u32, u32, i32, vp]),
+    "cmx_moe_token_unpermute_grad": (i32, [vp, u32, vp, u32, u32, i32p, f32p, vp, u32, f32p, u32, u32, u32, i32, i32, vp]),
     "catccos_ascend950_symmetric_bytes": (u64, []),
     "catccos_ascend950_dispatch_ffn_combine_workspace_bytes": (sz, [u32, u32, u32, u32, u32, i32]),
     "catccos_ascend950_dispatch_ffn_combine": (i32, [u32, vp, u64, u8p, u8p, u8p, u8p, u8p, u8p, u8p, u8p, u8p, u8p,

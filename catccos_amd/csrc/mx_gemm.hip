@@ -1964,6 +1964,9 @@ extern "C" int cmx_init(void) {
     if (int rc = preload_gating_kernels(); rc != CMX_OK) return rc;
     if (int rc = preload_gemv_kernels(); rc != CMX_OK) return rc;
     if (int rc = preload_moe_ffn_kernels(); rc != CMX_OK) return rc;
+    if (int rc = preload_fp8_quant_kernels(); rc != CMX_OK) return rc;
+    if (int rc = preload_fp8_gemm_kernels(); rc != CMX_OK) return rc;
+    if (int rc = preload_permute_kernels(); rc != CMX_OK) return rc;
     int cus = 0;
     if (int rc = cu_count(&cus); rc != CMX_OK) return rc;
     void* meta = nullptr;

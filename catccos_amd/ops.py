@@ -223,6 +223,86 @@ def mxfp4_gemv(x: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: str
                    (_OUT_DTYPE[out], m, n), n, OUT[out], m, n, k)
 
 
+def _fp8(fmt: str) -> int:
+    if fmt not in ("E4M3", "E5M2"):
+        raise ValueError("E4M3 or E5M2")
+    return FMT[fmt]
+
+
+def fp8_block_quant(x: torch.Tensor, fmt: str = "E4M3", square: bool = False, transposed: bool = False, pow2: bool = False):
+    """x [rows, cols] or [batch, rows, cols] bf16 / fp16 / fp32 -> (codes u8 [.., R, C rounded up to 16], scales fp32 [.., R or ceil(R/128), ceil(C/128)])
+    of z = x, or of its transpose: an fp32 scale for each 1 x 128 of z, or 128 x 128 if square; max |z| / 448 (E5M2: 57344), with pow2 the next power of
+    two.  Rows of codes end in zeros up to a multiple of 16 columns: that is the products' k."""
+    fmt = _fp8(fmt)
+    _here(x)
+    assert x.dim() in (2, 3)
+    batch, (rows, cols) = x.shape[0] if x.dim() == 3 else 1, x.shape[-2:]
+    _fits(batch | rows | cols)
+    if x.dim() == 2:
+        pitch, step = _pitch(x, cols), 0
+    elif x.is_contiguous():
+        pitch, step = cols, rows * cols
+    else:
+        step, pitch, one = x.stride()
+        assert one == 1 or cols <= 1, "rows must lie in one piece"
+        assert min(step, pitch) >= 0
+        pitch = pitch if rows > 1 else cols
+        _fits(pitch)
+    r, c = (cols, rows) if transposed else (rows, cols)
+    wide, blocks, s_rows = (c + 15) // 16 * 16, (c + 127) // 128, (r + 127) // 128 if square else r
+    head = (batch,) if x.dim() == 3 else ()
+    return _launch("cmx_fp8_block_quant", x, pitch, step, _TYPE[x.dtype], (torch.uint8, *head, r, wide), wide, (torch.float32, *head, s_rows, blocks), blocks,
+                   batch, rows, cols, fmt, 1 if square else 0, 1 if transposed else 0, 1 if pow2 else 0)
+
+
+def _scale_pitch(scale, rows: int, blocks: int) -> int:
+    assert scale.dtype == torch.float32 and scale.dim() == 2 and scale.shape[0] == rows and scale.shape[1] >= blocks, "scales"
+    return max(_pitch(scale, scale.shape[1]), blocks)
+
+
+def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16", c=None) -> torch.Tensor:
+    """a u8 [m, k] with a_scale fp32 [m, >= ceil(k/128)] times b u8 [n, k] with b_scale [ceil(n/128), ..] (a weight's 128 x 128) or [n, ..] (1 x 128,
+    as a weight's gradient has on both sides) -> c [m, n]; operands as fp8_block_quant makes them, k a multiple of 16."""
+    _here(a, a_scale, b, b_scale, c)
+    (m, k), (n, kb) = a.shape, b.shape
+    _fits(m | n | k)
+    assert a.dtype == b.dtype == torch.uint8 and k == kb
+    blocks = (k + 127) // 128
+    b_rows = 1 if n > 1 and b_scale.shape[0] == n else 128
+    ld_as, ld_bs = _scale_pitch(a_scale, m, blocks), _scale_pitch(b_scale, n if b_rows == 1 else (n + 127) // 128, blocks)
+    ldc = n
+    if c is None:
+        made = (_OUT_DTYPE[out], m, n)
+    else:
+        made = c
+        assert c.shape == (m, n) and c.dtype == _OUT_DTYPE[out]
+        ldc = _pitch(c, n)
+    got = _launch("cmx_fp8_block_gemm", a, _pitch(a, k), a_scale, ld_as, b, _pitch(b, k), b_scale, ld_bs, b_rows, made, ldc, m, n, k, _fp8(fmt), OUT[out])
+    return got if c is None else c
+
+
+def fp8_block_gmm(a, a_scale, b, b_scale, group_sizes, fmt: str = "E4M3", out: str = "bf16", c=None) -> torch.Tensor:
+    """fp8_block_gemm for ragged groups: a u8 [m_total, k], b u8 [G, n, k] with b_scale fp32 [G, ceil(n/128), ceil(k/128)], group_sizes int32 [G] on the
+    device -> [m_total, n].  Rows behind the groups are zeros in a new tensor and stay as they are in the caller's c."""
+    _here(a, a_scale, b, b_scale, group_sizes, c)
+    (m, k), (g, n, kb) = a.shape, b.shape
+    _fits(m | n | k | g)
+    blocks = (k + 127) // 128
+    assert a.dtype == b.dtype == torch.uint8 and k == kb and b.is_contiguous()
+    assert b_scale.dtype == torch.float32 and b_scale.shape == (g, (n + 127) // 128, blocks) and b_scale.is_contiguous()
+    assert group_sizes.dtype == torch.int32 and group_sizes.shape == (g,) and group_sizes.is_contiguous()
+    ldc = n
+    if c is None:
+        made = (_OUT_DTYPE[out], m, n)
+    else:
+        made = c
+        assert c.shape == (m, n) and c.dtype == _OUT_DTYPE[out]
+        ldc = _pitch(c, n)
+    got = _launch("cmx_fp8_block_gmm", a, _pitch(a, k), a_scale, _scale_pitch(a_scale, m, blocks), b, b_scale, made, ldc, group_sizes, g, m, n, k, _fp8(fmt), OUT[out],
+                  1 if c is None else 0)
+    return got if c is None else c
+
+
 def mx_to_k_major(src, src_scale, k: int, n: int):
     """codes [batch, k, n] (or [k, n]) with scales [batch, k/64, n, 2] -> K-contiguous codes [batch, n, k], scales [batch, n, k/32]."""
     _need_cuda(src, src_scale)
@@ -452,6 +532,49 @@ def moe_token_unpermute(y: torch.Tensor, src2sorted: torch.Tensor, probs: torch.
     _lib.check(lib.cmx_moe_token_unpermute(_p(y), y.stride(0), rows, _p(src2sorted), _p(probs), _p(out), h, t, h, top_k,
                                            _stream()))
     return out
+
+
+def _routes(src2sorted, top_k: int):
+    """Tokens of a table of routes, int32 [T * top_k] or [T, top_k]."""
+    assert src2sorted.dtype == torch.int32 and src2sorted.is_contiguous() and top_k >= 1 and src2sorted.numel() % top_k == 0
+    return src2sorted.numel() // top_k
+
+
+def moe_token_permute(x: torch.Tensor, src2sorted: torch.Tensor, top_k: int, out=None) -> torch.Tensor:
+    """Rows of x [T, h] (elements of 1, 2 or 4 bytes) to the experts' order: out[src2sorted[t * top_k + r]] = x[t]; src2sorted int32 [T * top_k].  A new
+    `out` has T * top_k rows, those of no route zero; in the caller's [rows, h] they stay as they are.  Destinations outside it are dropped routes."""
+    top_k = index(top_k)
+    _here(x, src2sorted, out)
+    t, h = x.shape
+    assert _routes(src2sorted, top_k) == t and x.element_size() in (1, 2, 4)
+    rows = t * top_k if out is None else out.shape[0]
+    _fits(t | h | rows | top_k)
+    if out is None:
+        return _launch("cmx_moe_token_permute", x, _pitch(x, h), src2sorted, (x.dtype, rows, h), h, rows, t, h, top_k, x.element_size(), 1)
+    assert out.dim() == 2 and out.shape[1] == h and out.dtype == x.dtype
+    _launch("cmx_moe_token_permute", x, _pitch(x, h), src2sorted, out, _pitch(out, h), rows, t, h, top_k, x.element_size(), 0)
+    return out
+
+
+def moe_token_permute_grad(dy: torch.Tensor, src2sorted: torch.Tensor, top_k: int) -> torch.Tensor:
+    """Gradient of moe_token_permute: dy [rows, h] bf16 / fp16 / fp32 -> [T, h], dx[t] = sum_r dy[src2sorted[t * top_k + r]] in fp32, rounded once."""
+    top_k = index(top_k)
+    _here(dy, src2sorted)
+    rows, h = dy.shape
+    t = _routes(src2sorted, top_k)
+    _fits(t | h | rows | top_k)
+    return _launch("cmx_moe_token_permute_grad", dy, _pitch(dy, h), rows, src2sorted, (dy.dtype, t, h), h, t, h, top_k, _TYPE[dy.dtype])
+
+
+def moe_token_unpermute_grad(dout: torch.Tensor, y: torch.Tensor, src2sorted: torch.Tensor, probs: torch.Tensor):
+    """Gradients of moe_token_unpermute(y, src2sorted, probs): dout [T, h] and y [rows, h] bf16 / fp16 / fp32, probs fp32 [T, top_k] -> (dy [rows, h],
+    dprobs fp32 [T, top_k]).  Rows of no route get zeros, dropped routes a zero."""
+    _here(dout, y, src2sorted, probs)
+    (t, h), (rows, hy), top_k = dout.shape, y.shape, probs.shape[1]
+    _fits(t | h | rows | top_k)
+    assert h == hy and dout.dtype == y.dtype and probs.shape[0] == t and probs.dtype == torch.float32 and probs.is_contiguous() and _routes(src2sorted, top_k) == t
+    return _launch("cmx_moe_token_unpermute_grad", dout, _pitch(dout, h), y, _pitch(y, h), rows, src2sorted, probs, (y.dtype, rows, h), h,
+                   (torch.float32, t, top_k), t, h, top_k, _TYPE[y.dtype], 1)
 
 
 def mxfp4_moe_ffn_workspace_bytes(m: int, n: int, top_k: int) -> int:

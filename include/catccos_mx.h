@@ -184,6 +184,43 @@ int cmx_mx_gmm(const uint8_t* a, uint32_t lda, const uint8_t* a_scale, uint32_t 
                cmx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * FP8 with an fp32 scale for each block of 128 (no counterpart in the reference, whose blocks of 32 have E8M0 scales): the form
+ * of models whose activations carry a scale for 1 x 128 elements and whose weights one for 128 x 128.
+ *
+ * cmx_fp8_block_quant makes such operands.  z = x, or x^T with `transposed`; blocks lie along the rows of z, of one row or, with `square`, of 128:
+ *   s = max(max |z| / most, 2^-126), most = 448 (E4M3) or 57344 (E5M2), rounded to fp32; with pow2 the least power of two that is no less;
+ *   code = the nearest value to the exact z / s, ties to even.
+ *   x        `batch` matrices [rows, cols] of `type` (CMX_OUT_BF16 / FP16 / FP32), pitch ld_x elements, x_step elements apart; elements' alignment
+ *   codes    u8, per matrix [R, C] = [rows, cols] ([cols, rows] if transposed), pitch ld_codes bytes, matrices R * ld_codes apart; every row ends in zeros up to
+ *            the next multiple of 16 columns, so that rows of any length are operands of the products below (their k is that multiple)
+ *   scales   fp32, per matrix [R or ceil(R / 128), ceil(C / 128)], pitch ld_scales elements, matrices that many rows apart
+ * The scale of a block that holds Inf or NaN is Inf or NaN, and its codes are 0x7F (NaN).  Rows of codes 16-byte aligned.
+ *
+ * cmx_fp8_block_gemm   c[m, n] = sum_kb (sa[m, kb] * sb[.., kb]) * sum_{k in block kb} a[m, k] * b[n, k]
+ *   a  codes [m, k], pitch lda bytes; a_scale [m, >= ceil(k / 128)], pitch ld_as elements
+ *   b  codes [n, k], pitch ldb bytes; b_scale [ceil(n / 128), ..] (b_rows = 128: a weight) or [n, ..] (b_rows = 1: scales by the row on both sides,
+ *      as a weight's gradient has them, from cmx_fp8_block_quant's transposed operands), pitch ld_bs elements
+ *   c  [m, n] of out_type, pitch ldc elements
+ * The gradient of a needs b quantised transposed; square blocks give the same codes and scales both ways, turned.
+ * The product of two scales is rounded to fp32, sums over blocks are fp32, c is rounded once.  In a block the matrix instruction aligns every eight
+ * consecutive products to the largest and drops what lies below 2^-13 of it (some 2^-16 of a result, also of an fp32 one).  As for cmx_mx_gemm a row's
+ * last bits can differ between calls with different m or n.
+ *
+ * cmx_fp8_block_gmm    the same over ragged groups of rows, as cmx_mx_gmm has them: group_sizes int32 [groups] on the device; b [groups, n, k] and
+ *   b_scale [groups, ceil(n / 128), ceil(k / 128)] dense.  Rows behind the groups, up to m_total, are left untouched, or cleared with zero_rest.  No workspace.
+ * k a multiple of 16; operand rows 16-byte aligned, at most 2^22 bytes apart.
+ * ---------------------------------------------------------------------------------------- */
+int cmx_fp8_block_quant(const void* x, uint32_t ld_x, uint64_t x_step, int type, uint8_t* codes, uint32_t ld_codes, float* scales,
+                        uint32_t ld_scales, uint32_t batch, uint32_t rows, uint32_t cols, int fmt, int square, int transposed, int pow2,
+                        cmx_stream_t stream);
+int cmx_fp8_block_gemm(const uint8_t* a, uint32_t lda, const float* a_scale, uint32_t ld_as, const uint8_t* b, uint32_t ldb,
+                       const float* b_scale, uint32_t ld_bs, uint32_t b_rows, void* c, uint32_t ldc, uint32_t m, uint32_t n,
+                       uint32_t k, int fmt, int out_type, cmx_stream_t stream);
+int cmx_fp8_block_gmm(const uint8_t* a, uint32_t lda, const float* a_scale, uint32_t ld_as, const uint8_t* b, const float* b_scale,
+                      void* c, uint32_t ldc, const int32_t* group_sizes, uint32_t groups, uint32_t m_total, uint32_t n, uint32_t k,
+                      int fmt, int out_type, int zero_rest, cmx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Grouped MXFP8 matmul with fused SwiGLU and MX requant (GMM1 of the FFN).
  * Replaces Ascend950AllToAllGmmKernel's AIC loop (ascend950_alltoall_gmm.hpp:193-323: gate and
  * up products per tile) + SwigluBf16RegBaseVf
@@ -410,6 +447,25 @@ int cmx_quant_scatter_zeroed(const void* x, uint32_t ld_x, const int32_t* src2so
 int cmx_moe_token_unpermute(const void* y, uint32_t ld_y, uint32_t rows, const int32_t* src2sorted,
                             const float* probs, void* out, uint32_t ld_out, uint32_t tokens, uint32_t hidden,
                             uint32_t top_k, cmx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The way to the experts' order without a quantiser, and the gradients of both ways (no counterpart in the reference).  With
+ * dst(t, r) = src2sorted[t * top_k + r]; a destination outside [0, rows) is a dropped route, and no two routes may have the same:
+ *   permute         out[dst(t, r)] = x[t]                        rows of any elements of 1, 2 or 4 bytes, codes and scales among them
+ *   permute_grad    dx[t] = sum_r dy[dst(t, r)]                  of `type` (CMX_OUT_BF16 / FP16 / FP32), in fp32 in the order of r, rounded once
+ *   unpermute_grad  of cmx_moe_token_unpermute(y, probs): dy[dst(t, r)] = probs[t, r] * dout[t] in fp32, rounded once; dprobs[t, r] = sum_h
+ *                   dout[t, h] * y[dst(t, r), h] in fp32, zero for a dropped route (dprobs fp32 [tokens, top_k])
+ * Rows of out and dy (`rows` of them) that no route is sent to are left as they were, or cleared with zero_rest.  Pitches in elements; elements' alignment.  No
+ * input may overlap an output.  top_k <= 64, tokens * top_k and rows < 2^31.
+ * ---------------------------------------------------------------------------------------- */
+int cmx_moe_token_permute(const void* x, uint32_t ld_x, const int32_t* src2sorted, void* out, uint32_t ld_out, uint32_t rows,
+                          uint32_t tokens, uint32_t hidden, uint32_t top_k, uint32_t element_bytes, int zero_rest,
+                          cmx_stream_t stream);
+int cmx_moe_token_permute_grad(const void* dy, uint32_t ld_dy, uint32_t rows, const int32_t* src2sorted, void* dx, uint32_t ld_dx,
+                               uint32_t tokens, uint32_t hidden, uint32_t top_k, int type, cmx_stream_t stream);
+int cmx_moe_token_unpermute_grad(const void* dout, uint32_t ld_dout, const void* y, uint32_t ld_y, uint32_t rows,
+                                 const int32_t* src2sorted, const float* probs, void* dy, uint32_t ld_dy, float* dprobs,
+                                 uint32_t tokens, uint32_t hidden, uint32_t top_k, int type, int zero_rest, cmx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * The routed FFN of a few tokens on MXFP4 expert weights, activations in bf16 (W4A16): the FFN below at decode, with
