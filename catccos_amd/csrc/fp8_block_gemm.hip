@@ -318,6 +318,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
     constexpr uint32_t kScaleRows = TM + (ROW_SCALES ? TN : 0), kScaleBase = SLOTS * kSlot, kScaleHalf = kScaleRows * kScaleSpan * 4;
     static_assert(TN % (8 * NW) == 0 && TM % (8 * NW) == 0 && (8 * NW) % 16 == 0, "loads of whole rows, the same piece in all of a lane's");
     static_assert(128 % (TN / WN) == 0, "a wavefront's columns share a scale");
+    static_assert(2 * kLoads <= FN * FM && FM >= 3, "loads behind every other product; a fragment of b is free again when its last sums are added");
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = same(tid >> 6), wn = wave % WN, wm = wave / WN, r16 = lane & 15u, quarter = lane >> 4;
     Work w;
     if (!locate<TM>(p, blockIdx.x, w, true)) return;
@@ -340,10 +341,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
         off[i] = (i < kBLoads ? min(r, n_rows - 1) * p.ldb : min(r - TN, w.rows - 1) * p.lda) + 16 * my_piece;
     }
     const uint32_t last = p.blocks - 1, behind = last * kBlockK + 16 * my_piece < p.k ? 0u : 0x80000000u;      // pieces behind K, in its last block
-    const auto issue = [&](uint32_t kb, uint32_t slot) {
-        const uint32_t gone = kb == last ? behind : 0u;
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) dma16(lds0 + slot * kSlot + (NW * i + wave) * 1024, off[i] | gone, i < kBLoads ? b_buf : a_buf, kb * kBlockK);
+    // load i of block kb; past the last block zeros come without a look at memory, so that every block counts the same loads
+    const auto gone = [&](uint32_t kb) -> uint32_t { return kb < last ? 0u : (kb == last ? behind : 0x80000000u); };
+    const auto issue = [&](uint32_t kb, uint32_t slot, uint32_t i, uint32_t gone) {
+        dma16(lds0 + slot * kSlot + (NW * i + wave) * 1024, off[i] | gone, i < kBLoads ? b_buf : a_buf, kb * kBlockK);
     };
     // scales of blocks span * kScaleSpan .. + kScaleSpan, [block][row], into half span % 2; a thread has some rows' four blocks
     constexpr uint32_t kPieces = kScaleRows * (kScaleSpan / 4), kMine = (kPieces + NT - 1) / NT;
@@ -381,58 +382,74 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
     for (uint32_t i = 0; i < FN; ++i)
 #pragma unroll
         for (uint32_t j = 0; j < FM; ++j) sum[i][j] = (v4f){0, 0, 0, 0};
-    const auto fragment = [&](const uint8_t* slot, uint32_t row) -> v8i {
-        const uint8_t* const r = slot + row * kBlockK;
-        const v4i lo = *reinterpret_cast<const v4i*>(r + 16 * place_of(row, quarter)), hi = *reinterpret_cast<const v4i*>(r + 16 * place_of(row, quarter + 4));
-        return (v8i){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    // a fragment's rows are 16 apart from those of the next: their pieces lie at the same places, and the second 64 bytes at the first's with one bit turned
+    const uint32_t in_rows = r16 * kBlockK + 16 * place_of(r16, quarter);
+    const uint32_t b_lo = wn * (TN / WN) * kBlockK + in_rows, a_lo = (TN + wm * (TM / WM)) * kBlockK + in_rows;
+    const auto fragment = [&](uint32_t lo, uint32_t i) -> v8i {
+        typedef __attribute__((address_space(3))) const v4i* lds_v4i;
+        const v4i x = *(lds_v4i)(uintptr_t)(lo + i * (16 * kBlockK)), y = *(lds_v4i)(uintptr_t)((lo ^ 64u) + i * (16 * kBlockK));
+        return (v8i){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     };
 
     fetch_scales(0);
     place_scales(0);
 #pragma unroll
     for (uint32_t d = 0; d + 1 < SLOTS; ++d)
-        if (d < p.blocks) issue(d, d);
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) issue(d, d, i, gone(d));
     uint32_t slot = 0;
     float sb = ROW_SCALES ? 0.0f : b_scale[0];
     for (uint32_t kb = 0; kb < p.blocks; ++kb) {
         // block kb has arrived for all, and all have read block kb - 1
-        if (SLOTS == 2 || kb + 1 >= p.blocks) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((SLOTS - 2) * kLoads) : "memory");
-        if (kb + SLOTS - 1 < p.blocks) issue(kb + SLOTS - 1, slot == 0 ? SLOTS - 1 : slot - 1);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((SLOTS - 2) * kLoads) : "memory");
+        const uint32_t next_slot = slot == 0 ? SLOTS - 1 : slot - 1, next_gone = gone(kb + SLOTS - 1);
         const uint32_t span = kb / kScaleSpan, in_span = kb % kScaleSpan;
         const bool more = (span + 1) * kScaleSpan < p.blocks;
         if (in_span == 1 && more) fetch_scales(span + 1);
-        const uint8_t* const at = smem + slot * kSlot;
+        const uint32_t at = lds0 + slot * kSlot;
         const float* const scales = reinterpret_cast<const float*>(smem + kScaleBase + (span & 1u) * kScaleHalf) + in_span * kScaleRows;
-        v8i a[FM];
+        v8i a[FM], b[2];
         float s[FM];
+        v4f part[4], rs[3];
+        const uint32_t b_row = wn * (TN / WN), a_row = wm * (TM / WM) + r16, b_at = at + b_lo, a_at = at + a_lo;
+        const auto b_fragment = [&](uint32_t i) {
+            b[i & 1] = fragment(b_at, i);
+            if constexpr (ROW_SCALES) rs[i % 3] = *reinterpret_cast<const v4f*>(scales + TM + b_row + 16 * i + 4 * quarter);
+        };
+        b_fragment(0);
 #pragma unroll
         for (uint32_t j = 0; j < FM; ++j) {
-            const uint32_t row = wm * (TM / WM) + 16 * j + r16;
-            a[j] = fragment(at + TN * kBlockK, row);
-            s[j] = scales[row];
+            a[j] = fragment(a_at, j);
+            s[j] = scales[a_row + 16 * j];
             if constexpr (!ROW_SCALES) s[j] *= sb;
         }
+        __builtin_amdgcn_sched_barrier(0);
+        const auto add = [&](uint32_t x) {
+            const uint32_t i = x / FM, j = x % FM;
+            asm volatile("" : "+v"(part[x % 4]));                      // (not in AGPRs, from which the vector unit would have to copy it)
 #pragma unroll
-        for (uint32_t i = 0; i < FN; ++i) {
-            const uint32_t row = wn * (TN / WN) + 16 * i;
-            const v8i b = fragment(at, row + r16);
-            v4f rs;
-            if constexpr (ROW_SCALES) rs = *reinterpret_cast<const v4f*>(scales + TM + row + 4 * quarter);
-#pragma unroll
-            for (uint32_t j = 0; j < FM; ++j) {
-                const v4f part = block_product<FMT>(b, a[j]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if constexpr (ROW_SCALES) sum[i][j][r] = __builtin_fmaf(part[r], rs[r] * s[j], sum[i][j][r]);
-                    else sum[i][j][r] = __builtin_fmaf(part[r], s[j], sum[i][j][r]);
-                }
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (ROW_SCALES) sum[i][j][r] = __builtin_fmaf(part[x % 4][r], rs[i % 3][r] * s[j], sum[i][j][r]);
+                else sum[i][j][r] = __builtin_fmaf(part[x % 4][r], s[j], sum[i][j][r]);
             }
+            asm volatile("" : "+v"(sum[i][j]));                        // (used here: the compiler would put all multiply-adds behind all products)
+        };
+        // a product, the multiply-adds of the one three before, its share of the loads: in this order
+#pragma unroll
+        for (uint32_t x = 0; x < FN * FM; ++x) {
+            part[x % 4] = block_product<FMT>(b[x / FM & 1], a[x % FM]);
+            if (x >= 3) add(x - 3);
+            if (x % FM == 0 && x / FM + 1 < FN) b_fragment(x / FM + 1);
+            if (x % 2 == 1 && x / 2 < kLoads) issue(kb + SLOTS - 1, next_slot, x / 2, next_gone);
+            __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (uint32_t x = FN * FM - 3; x < FN * FM; ++x) add(x);
         if (in_span == 4 && more) place_scales(span + 1);
         if constexpr (!ROW_SCALES) sb = b_scale[min(kb + 1, last)];
         slot = slot + 1 < SLOTS ? slot + 1 : 0;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // the loads past the end, before the LDS changes hands
     const uint32_t size = p.out_type == CMX_OUT_FP32 ? 4 : 2;
 #pragma unroll
     for (uint32_t j = 0; j < FM; ++j) {
