@@ -71,7 +71,8 @@ SIGNATURES = {
     "cmx_mxfp4_moe_ffn_workspace_bytes": (sz, [u32, u32, u32]),
     "cmx_mxfp4_moe_ffn": (i32, [vp, i32p, f32p, u8p, u8p, u8p, u8p, vp, u8p, u32, u32, u32, u32, u32, vp]),
     "cmx_fp8_block_quant": (i32, [vp, u32, u64, i32, u8p, u32, f32p, u32, u32, u32, u32, i32, i32, i32, i32, vp]),
-    "cmx_fp8_block_gemm": (i32, [u8p, u32, f32p, u32, u8p, u32, f32p, u32, u32, vp, u32, u32, u32, u32, i32, i32, vp]),
+    "cmx_fp8_block_gemm": (i32, [u8p, u32, f32p, u32, u8p, u32, f32p, u32, u32, vp, u32, u32, u32, u32, i32, i32, vp, vp]),
+    "cmx_fp8_block_gemm_workspace_bytes": (sz, [u32, u32, u32]),
     "cmx_fp8_block_gmm": (i32, [u8p, u32, f32p, u32, u8p, f32p, vp, u32, i32p, u32, u32, u32, u32, i32, i32, i32, vp]),
     "cmx_moe_token_permute": (i32, [vp, u32, i32p, vp, u32, u32, u32, u32, u32, u32, i32, vp]),
     "cmx_moe_token_permute_grad": (i32, [vp, u32, u32, i32p, vp, u32, u32, u32, u32, i32, vp]),

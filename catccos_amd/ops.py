@@ -260,10 +260,16 @@ def _scale_pitch(scale, rows: int, blocks: int) -> int:
     return max(_pitch(scale, scale.shape[1]), blocks)
 
 
-def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16", c=None) -> torch.Tensor:
+def fp8_block_gemm_workspace_bytes(m: int, n: int, k: int) -> int:
+    m, n, k = index(m), index(n), index(k)
+    _fits(m | n | k)
+    return _lib.load().cmx_fp8_block_gemm_workspace_bytes(m, n, k)
+
+
+def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16", c=None, workspace=None) -> torch.Tensor:
     """a u8 [m, k] with a_scale fp32 [m, >= ceil(k/128)] times b u8 [n, k] with b_scale [ceil(n/128), ..] (a weight's 128 x 128) or [n, ..] (1 x 128,
     as a weight's gradient has on both sides) -> c [m, n]; operands as fp8_block_quant makes them, k a multiple of 16."""
-    _here(a, a_scale, b, b_scale, c)
+    _here(a, a_scale, b, b_scale, c, workspace)
     (m, k), (n, kb) = a.shape, b.shape
     _fits(m | n | k)
     assert a.dtype == b.dtype == torch.uint8 and k == kb
@@ -277,7 +283,13 @@ def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16",
         made = c
         assert c.shape == (m, n) and c.dtype == _OUT_DTYPE[out]
         ldc = _pitch(c, n)
-    got = _launch("cmx_fp8_block_gemm", a, _pitch(a, k), a_scale, ld_as, b, _pitch(b, k), b_scale, ld_bs, b_rows, made, ldc, m, n, k, _fp8(fmt), OUT[out])
+    if m > 16 or workspace is not None:                                # (a few rows never need one)
+        need = fp8_block_gemm_workspace_bytes(m, n, k)
+        if workspace is None:
+            workspace = _empty(a, torch.uint8, need) if need else None
+        else:
+            assert workspace.is_contiguous() and workspace.nbytes >= need
+    got = _launch("cmx_fp8_block_gemm", a, _pitch(a, k), a_scale, ld_as, b, _pitch(b, k), b_scale, ld_bs, b_rows, made, ldc, m, n, k, _fp8(fmt), OUT[out], workspace)
     return got if c is None else c
 
 

@@ -201,6 +201,8 @@ int cmx_mx_gmm(const uint8_t* a, uint32_t lda, const uint8_t* a_scale, uint32_t 
  *   b  codes [n, k], pitch ldb bytes; b_scale [ceil(n / 128), ..] (b_rows = 128: a weight) or [n, ..] (b_rows = 1: scales by the row on both sides,
  *      as a weight's gradient has them, from cmx_fp8_block_quant's transposed operands), pitch ld_bs elements
  *   c  [m, n] of out_type, pitch ldc elements
+ *   workspace  >= cmx_fp8_block_gemm_workspace_bytes(m, n, k) bytes on this device (0 for most sizes), 16-byte aligned: where few tiles would leave CUs
+ *      idle, workgroups share K and their sums meet there.  With NULL none is used
  * The gradient of a needs b quantised transposed; square blocks give the same codes and scales both ways, turned.
  * The product of two scales is rounded to fp32, sums over blocks are fp32, c is rounded once.  In a block the matrix instruction aligns every eight
  * consecutive products to the largest and drops what lies below 2^-13 of it (some 2^-16 of a result, also of an fp32 one).  As for cmx_mx_gemm a row's
@@ -213,9 +215,10 @@ int cmx_mx_gmm(const uint8_t* a, uint32_t lda, const uint8_t* a_scale, uint32_t 
 int cmx_fp8_block_quant(const void* x, uint32_t ld_x, uint64_t x_step, int type, uint8_t* codes, uint32_t ld_codes, float* scales,
                         uint32_t ld_scales, uint32_t batch, uint32_t rows, uint32_t cols, int fmt, int square, int transposed, int pow2,
                         cmx_stream_t stream);
+size_t cmx_fp8_block_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
 int cmx_fp8_block_gemm(const uint8_t* a, uint32_t lda, const float* a_scale, uint32_t ld_as, const uint8_t* b, uint32_t ldb,
                        const float* b_scale, uint32_t ld_bs, uint32_t b_rows, void* c, uint32_t ldc, uint32_t m, uint32_t n,
-                       uint32_t k, int fmt, int out_type, cmx_stream_t stream);
+                       uint32_t k, int fmt, int out_type, void* workspace, cmx_stream_t stream);
 int cmx_fp8_block_gmm(const uint8_t* a, uint32_t lda, const float* a_scale, uint32_t ld_as, const uint8_t* b, const float* b_scale,
                       void* c, uint32_t ldc, const int32_t* group_sizes, uint32_t groups, uint32_t m_total, uint32_t n, uint32_t k,
                       int fmt, int out_type, int zero_rest, cmx_stream_t stream);

@@ -16,7 +16,7 @@ def test_host_tensors():
 
 # calls that are whole; the addresses are never reached
 QUANT = dict(x=4096, ld_x=300, x_step=0, type=0, codes=4096, ld_codes=304, scales=4096, ld_scales=3, batch=1, rows=5, cols=300, fmt=0, square=0, transposed=0, pow2=0, stream=None)
-GEMM = dict(a=4096, lda=256, a_scale=4096, ld_as=2, b=4096, ldb=256, b_scale=4096, ld_bs=2, b_rows=128, c=4096, ldc=8, m=2, n=8, k=256, fmt=0, out_type=0, stream=None)
+GEMM = dict(a=4096, lda=256, a_scale=4096, ld_as=2, b=4096, ldb=256, b_scale=4096, ld_bs=2, b_rows=128, c=4096, ldc=8, m=2, n=8, k=256, fmt=0, out_type=0, workspace=None, stream=None)
 GMM = dict(a=4096, lda=256, a_scale=4096, ld_as=2, b=4096, b_scale=4096, c=4096, ldc=8, sizes=4096, groups=3, m=2, n=8, k=256, fmt=0, out_type=0, zero_rest=0, stream=None)
 
 
@@ -44,7 +44,7 @@ PRODUCT = [(dict(a=None), "null pointer"), (dict(a_scale=None), "null pointer"),
            (dict(lda=(1 << 22) + 16), "2^22 bytes apart"), (dict(m=(1 << 31) - 1, n=1 << 24, ldc=1 << 24), "too many tiles")]
 
 
-@pytest.mark.parametrize("change,message", PRODUCT + [(dict(ldb=240), "pitch"), (dict(ld_bs=1), "pitch"), (dict(b_rows=64), "every row or every 128"), (dict(ldb=264), "16-byte")])
+@pytest.mark.parametrize("change,message", PRODUCT + [(dict(ldb=240), "pitch"), (dict(ld_bs=1), "pitch"), (dict(b_rows=64), "every row or every 128"), (dict(ldb=264), "16-byte"), (dict(workspace=4104), "workspace")])
 def test_gemm_refuses_before_a_launch(change, message):
     _refused_product("cmx_fp8_block_gemm", {**GEMM, **change}, message)
 
