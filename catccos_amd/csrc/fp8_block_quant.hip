@@ -2,8 +2,7 @@
 //
 //   s = max(max |z| / most, 2^-126), or the least power of two that is no less;  code = the nearest value to z / s, ties to even
 //
-// The quotient is that of the exact z / s, not of its fp32 value: z * (1 / s) is off by some 2^-22 of itself, and where that leaves it next to a
-// border between two codes (a few values in 10^5) the sign of z - border * s, one fused multiply-add, decides.
+// The quotient is that of the exact z / s, not of its fp32 value.
 // Bound by memory: 3 bytes to a 16-bit element.
 #include <type_traits>
 
@@ -27,14 +26,20 @@ struct Fp8QuantArgs {
     uint32_t out_rows, scale_rows, blocks;
     uint32_t vec;                                    // rows of x are whole 16-byte pieces
     uint32_t pow2;
+    uint32_t block_part;                             // 65536 / blocks, rounded up, for few blocks
 };
 
+template <bool STREAM, class V>
+__device__ __forceinline__ V load_piece(const uint8_t* p, uint32_t i = 0) {
+    return STREAM ? __builtin_nontemporal_load(reinterpret_cast<const V*>(p) + i) : reinterpret_cast<const V*>(p)[i];
+}
+
 // eight consecutive elements of type T, `n` of them there, the others zero
-template <int TYPE>
+template <int TYPE, bool STREAM = false>
 __device__ __forceinline__ void load8(const uint8_t* p, bool whole, uint32_t n, float (&v)[8]) {
     if constexpr (TYPE == CMX_OUT_FP32) {
         if (whole) {
-            const v4f lo = reinterpret_cast<const v4f*>(p)[0], hi = reinterpret_cast<const v4f*>(p)[1];
+            const v4f lo = load_piece<STREAM, v4f>(p), hi = load_piece<STREAM, v4f>(p, 1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) { v[i] = lo[i]; v[4 + i] = hi[i]; }
         } else {
@@ -45,7 +50,7 @@ __device__ __forceinline__ void load8(const uint8_t* p, bool whole, uint32_t n, 
     }
     uint32_t w[4];
     if (whole) {
-        const v4i d = *reinterpret_cast<const v4i*>(p);
+        const v4i d = load_piece<STREAM, v4i>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = (uint32_t)d[i];
     } else {
@@ -73,10 +78,14 @@ struct BlockScale {
     float s, inverse;
     bool finite;
     __device__ __forceinline__ BlockScale(uint32_t amax_bits, uint32_t pow2) {
-        constexpr float kMost = FMT == CMX_FMT_E5M2 ? 57344.0f : 448.0f;
+        constexpr float kMost = FMT == CMX_FMT_E5M2 ? 57344.0f : 448.0f, kPart = 1.0f / kMost;
         finite = amax_bits < kInfBits;
-        s = __uint_as_float(amax_bits) / kMost;                       // (rounded to nearest; Inf and NaN stay what they are)
+        const float amax = __uint_as_float(amax_bits);
+        s = amax;                                                     // (Inf and NaN are scales themselves)
         if (finite) {
+            // the quotient rounded to nearest: what amax * (1 / most) is off by is known exactly, and small
+            s = amax * kPart;
+            s = __builtin_fmaf(__builtin_fmaf(-s, kMost, amax), kPart, s);
             // amax / most is no closer above a power of two than its fp32 quotient can tell: 448 and 57344 are 1.75 * 2^i, and of the amax right above
             // such a value the quotient is 1 + 2^-23 / 1.75
             if (pow2) s = __uint_as_float((__float_as_uint(s) + 0x007FFFFFu) & 0xFF800000u);
@@ -84,24 +93,8 @@ struct BlockScale {
         }
         inverse = __builtin_amdgcn_rcpf(s);
     }
+    __device__ __forceinline__ BlockScale(float scale, float inv, bool is_finite) : s(scale), inverse(inv), finite(is_finite) {}
 };
-
-// |q| is within 4 units of fp32's last place of a border between codes, or of a code below the normal ones (their borders have fewer bits)
-template <int FMT>
-__device__ __forceinline__ bool near_border(float q) {
-    constexpr uint32_t kUnder = FMT == CMX_FMT_E5M2 ? 20 : 19;       // bits under the border's own
-    constexpr uint32_t kNormal = (FMT == CMX_FMT_E5M2 ? 127 - 14 : 127 - 6) << 23;
-    const uint32_t u = magnitude(q) + 4;
-    return (u & ((1u << kUnder) - 1)) <= 8 && ((u >> kUnder & 1) != 0 || u < kNormal + 8);
-}
-// q = z / s to within 4 units, next to the border b: moved to the side of b where z / s lies, or onto it
-__device__ __forceinline__ float settled(float q, float z, float s, uint32_t under) {
-    const float b = __uint_as_float((__float_as_uint(q) + 4) & ~((1u << under) - 1));
-    const float lift = s < 0x1p-60f ? 0x1p100f : 1.0f;                // (what is left of a small z would lie below fp32's least value)
-    const float rest = __builtin_fmaf(-b, s * lift, z * lift);        // its sign is exact
-    if (rest == 0.0f) return b;
-    return __uint_as_float(__float_as_uint(b) + ((rest < 0.0f) == (z < 0.0f) ? 1u : ~0u));
-}
 
 template <int FMT>
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
@@ -114,24 +107,26 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
     return cvt_pk_e4m3(c, d, w, true);
 }
 
-// z into the quotients that the hardware's cast rounds to the codes of z / s
+// z into numbers that the hardware's cast rounds to the codes of the exact z / s.  Codes and the borders between them have at most 4 significant bits (E5M2 3): b is the value
+// of so many bits that z * (1 / s) is next to, and if z / s is not b it lies on the side of b that the sign of z - b * s says, one fused multiply-add; the cast gets b
+// moved to that side by 2^-10 of itself, which crosses nothing.  (z - b * s is a multiple of 2^-28 of z, so that 2^30 times it exceeds the 2^-10.)
+// 8 operations an element for all of them: a look for values next to a border first takes 5, but of bf16 elements so many lie on one (3/4 and 3/2 of a maximum are borders) that
+// two wavefronts in five went on (8192 x 7168: 25 vector operations an element and 35.6 us, so 33).
 template <int FMT, int N>
-__device__ __forceinline__ void quotients(float (&z)[N], const BlockScale<FMT>& b) {
+__device__ __forceinline__ void quotients(float (&z)[N], BlockScale<FMT> b) {
     constexpr uint32_t kUnder = FMT == CMX_FMT_E5M2 ? 20 : 19;
-    float q[N];
-    bool near = false;
+    if (b.s < 0x1p-60f) {                                              // (what is left of a small z would lie below fp32's least value)
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] *= 0x1p100f;
+        b.s *= 0x1p100f;
+        b.inverse *= 0x1p-100f;
+    }
+    const float far = b.inverse * 0x1p30f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        q[i] = z[i] * b.inverse;
-        near |= near_border<FMT>(q[i]);
+        const float q = __uint_as_float((__float_as_uint(z[i] * b.inverse) + (1u << (kUnder - 1))) & ~((1u << kUnder) - 1)), step = fabsf(q) * 0x1p-10f;
+        z[i] = q + __builtin_amdgcn_fmed3f(__builtin_fmaf(-q, b.s, z[i]) * far, -step, step);
     }
-    if (near) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (near_border<FMT>(q[i]) && z[i] != 0.0f) q[i] = settled(q[i], z[i], b.s, kUnder);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = q[i];
 }
 
 template <int FMT>
@@ -149,24 +144,28 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xF, 0xF, false));
 }
 
-constexpr uint32_t kRowBlocks = 2;                   // blocks of a 16-lane team
+constexpr uint32_t kRowBlocks = 4;                   // blocks of a 16-lane team
 
-// Blocks of 1 x 128 of x itself: 16 lanes to a block, eight elements to a lane, kRowBlocks blocks in flight.
-template <int TYPE, int FMT>
+// Blocks of 1 x 128 of x itself: 16 lanes to a block, eight elements to a lane, kRowBlocks blocks in flight.  8192 x 7168 bf16: 30.9 us, 5.8 TB/s.
+// STREAM: past the caches, both ways.  From 96 MiB of x on, which the caches hold no longer than it takes to read them (8192 x 7168: 30.9 us, reading alone 32.8, neither
+// 34.6); below that a product that follows finds the codes nearer.
+template <int TYPE, int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const Fp8QuantArgs a) {
     constexpr uint32_t kSize = TYPE == CMX_OUT_FP32 ? 4 : 2, kTeams = 256 / 16;
-    const uint32_t lane = threadIdx.x & 15u;
-    const uint64_t total = (uint64_t)a.rows * a.blocks, first = (uint64_t)blockIdx.x * (kTeams * kRowBlocks) + threadIdx.x / 16;
+    const uint32_t lane = threadIdx.x & 15u, team = threadIdx.x / 16;
+    // blocks are numbered row by row; the workgroup's first one is found by a division, the others by steps from there
+    const uint32_t total = a.rows * a.blocks, first = blockIdx.x * (kTeams * kRowBlocks), row0 = first / a.blocks, blk0 = first - row0 * a.blocks;
     const uint8_t* const x = a.x + blockIdx.y * a.x_step;
     float v[kRowBlocks][8];
     uint32_t row[kRowBlocks], blk[kRowBlocks];
 #pragma unroll
     for (uint32_t i = 0; i < kRowBlocks; ++i) {
-        const uint64_t at = first + i * kTeams < total ? first + i * kTeams : total - 1;
-        row[i] = (uint32_t)(at / a.blocks);
-        blk[i] = (uint32_t)(at - (uint64_t)row[i] * a.blocks);
+        const uint32_t at = blk0 + min(team + i * kTeams, total - 1 - first);
+        const uint32_t down = a.blocks > kTeams * kRowBlocks ? (at >= a.blocks ? 1u : 0u) : (at * a.block_part) >> 16;      // at / a.blocks
+        row[i] = row0 + down;
+        blk[i] = at - down * a.blocks;
         const uint32_t col = blk[i] * kBlock + 8 * lane, n = col < a.cols ? a.cols - col : 0;
-        load8<TYPE>(x + row[i] * a.ld_x + (size_t)col * kSize, a.vec && n >= 8, n, v[i]);
+        load8<TYPE, STREAM>(x + row[i] * a.ld_x + (size_t)col * kSize, a.vec && n >= 8, n, v[i]);
     }
 #pragma unroll
     for (uint32_t i = 0; i < kRowBlocks; ++i) {
@@ -176,7 +175,7 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const Fp8QuantArgs 
         const BlockScale<FMT> b(max16(amax), a.pow2);
         const uint2 c = codes8<FMT>(v[i], b);
         const uint32_t col = blk[i] * kBlock + 8 * lane;
-        if (first + i * kTeams >= total) continue;
+        if (first + team + i * kTeams >= total) continue;
         const size_t r = (size_t)blockIdx.y * a.rows + row[i];
         if (col < a.out_wide) {
             uint2 w = c;
@@ -185,7 +184,9 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const Fp8QuantArgs 
                 const uint64_t keep = n == 0 ? 0 : ~0ull >> (64 - 8 * n);
                 w = make_uint2(c.x & (uint32_t)keep, c.y & (uint32_t)(keep >> 32));
             }
-            *reinterpret_cast<uint2*>(a.codes + r * a.ld_codes + col) = w;
+            v2i* const to = reinterpret_cast<v2i*>(a.codes + r * a.ld_codes + col);
+            if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(v2i, w), to);
+            else *to = __builtin_bit_cast(v2i, w);
         }
         if (lane == 0) a.scales[r * a.ld_scales + blk[i]] = b.s;
     }
@@ -196,9 +197,11 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const Fp8QuantArgs 
 template <int TYPE, int FMT, bool SQUARE, bool TURNED>
 __global__ __launch_bounds__(256) void fp8_quant_tile_kernel(const Fp8QuantArgs a) {
     static_assert(SQUARE || TURNED, "rows of x itself have a kernel of their own");
-    constexpr uint32_t kSize = TYPE == CMX_OUT_FP32 ? 4 : 2, kPitch = kBlock + 8;
+    constexpr uint32_t kSize = TYPE == CMX_OUT_FP32 ? 4 : 2;
     __shared__ uint32_t s_max[16][kBlock + 4];
-    __shared__ __attribute__((aligned(16))) uint8_t s_codes[TURNED ? kBlock * kPitch : 16];
+    __shared__ float s_scale[2][kBlock];
+    // row r of codes holds its 8-byte piece p at place p ^ (r / 8): the 16 threads that write pieces of rows 8 apart meet different banks
+    __shared__ __attribute__((aligned(16))) uint8_t s_codes[TURNED ? kBlock * kBlock : 16];
     const uint32_t tx = threadIdx.x & 15u, ty = threadIdx.x >> 4;      // column and row of the thread's 8 x 8
     const uint32_t col0 = blockIdx.x * kBlock, row0 = blockIdx.y * kBlock, col = col0 + 8 * tx, row = row0 + 8 * ty;
     const uint8_t* const x = a.x + blockIdx.z * a.x_step;
@@ -252,24 +255,31 @@ __global__ __launch_bounds__(256) void fp8_quant_tile_kernel(const Fp8QuantArgs 
                 float t[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t[i] = v[i][j];
-                *reinterpret_cast<uint2*>(s_codes + (8 * tx + j) * kPitch + 8 * ty) = codes8<FMT>(t, b);
+                *reinterpret_cast<uint2*>(s_codes + (8 * tx + j) * kBlock + 8 * (ty ^ tx)) = codes8<FMT>(t, b);
             }
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) s_max[ty][8 * tx + j] = most[j];
         __syncthreads();
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
+        if (threadIdx.x < kBlock) {                                    // a thread to a column
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) m = max(m, s_max[i][8 * tx + j]);
+            for (int i = 0; i < 16; ++i) m = max(m, s_max[i][threadIdx.x]);
             const BlockScale<FMT> b(m, a.pow2);
+            s_scale[0][threadIdx.x] = b.s;
+            s_scale[1][threadIdx.x] = b.inverse;
+            if (col0 + threadIdx.x < a.cols) a.scales[(s0 + col0 + threadIdx.x) * a.ld_scales + blockIdx.y] = b.s;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const float scale = s_scale[0][8 * tx + j];
+            const BlockScale<FMT> b(scale, s_scale[1][8 * tx + j], magnitude(scale) < kInfBits);
             float t[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) t[i] = v[i][j];
-            *reinterpret_cast<uint2*>(s_codes + (8 * tx + j) * kPitch + 8 * ty) = codes8<FMT>(t, b);
-            if (ty == 0 && col + j < a.cols) a.scales[(s0 + col + j) * a.ld_scales + blockIdx.y] = b.s;
+            *reinterpret_cast<uint2*>(s_codes + (8 * tx + j) * kBlock + 8 * (ty ^ tx)) = codes8<FMT>(t, b);
         }
     }
     if constexpr (TURNED) {
@@ -280,8 +290,9 @@ __global__ __launch_bounds__(256) void fp8_quant_tile_kernel(const Fp8QuantArgs 
         for (uint32_t i = 0; i < 4; ++i) {
             const uint32_t r = threadIdx.x / 8 + 32 * i;
             if (col0 + r >= a.cols || out_col >= a.out_wide) continue;
-            const uint2* const from = reinterpret_cast<const uint2*>(s_codes + r * kPitch + 16 * piece);
-            uint64_t w[2] = {(uint64_t)from[0].x | (uint64_t)from[0].y << 32, (uint64_t)from[1].x | (uint64_t)from[1].y << 32};
+            uint64_t w[2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) w[h] = *reinterpret_cast<const uint64_t*>(s_codes + r * kBlock + 8 * ((2 * piece + h) ^ (r >> 3)));
             const uint32_t left = a.out_cols > out_col ? a.out_cols - out_col : 0;       // (behind them zeros, also in a block that is not finite)
             if (left < 16) {
                 w[1] = left <= 8 ? 0 : w[1] & (~0ull >> (128 - 8 * left));
@@ -297,8 +308,9 @@ template <int TYPE, int FMT>
 int launch(const Fp8QuantArgs& a, uint32_t batch, bool square, bool turned, hipStream_t s) {
     if (!square && !turned) {
         const uint64_t groups = ((uint64_t)a.rows * a.blocks + 16 * kRowBlocks - 1) / (16 * kRowBlocks);
-        CMX_REQUIRE(fits_grid(groups, 256), "too many elements");
-        hipLaunchKernelGGL((fp8_quant_rows_kernel<TYPE, FMT>), dim3((uint32_t)groups, batch), dim3(256), 0, s, a);
+        CMX_REQUIRE((uint64_t)a.rows * a.blocks < (1ull << 31) && fits_grid(groups, 256), "too many elements");
+        const bool stream = (uint64_t)batch * a.rows * a.cols * (TYPE == CMX_OUT_FP32 ? 4 : 2) >= 96ull << 20;
+        hipLaunchKernelGGL((stream ? fp8_quant_rows_kernel<TYPE, FMT, true> : fp8_quant_rows_kernel<TYPE, FMT, false>), dim3((uint32_t)groups, batch), dim3(256), 0, s, a);
     } else {
         const uint32_t bx = ceil_div(a.cols, kBlock), by = ceil_div(a.rows, kBlock);
         CMX_REQUIRE(by <= 65535u && fits_grid(bx, 256), "too many rows or columns");
@@ -320,7 +332,7 @@ int launch(const Fp8QuantArgs& a, uint32_t batch, int fmt, bool square, bool tur
 
 int cmx::preload_fp8_quant_kernels() {
     hipFuncAttributes attr;
-    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::fp8_quant_rows_kernel<CMX_OUT_BF16, CMX_FMT_E4M3>)));
+    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::fp8_quant_rows_kernel<CMX_OUT_BF16, CMX_FMT_E4M3, false>)));
     return CMX_OK;
 }
 
@@ -341,7 +353,7 @@ extern "C" int cmx_fp8_block_quant(const void* x, uint32_t ld_x, uint64_t x_step
     CMX_REQUIRE(reinterpret_cast<uintptr_t>(x) % size == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0, "pointers must be aligned to their elements");
     CMX_REQUIRE(aligned16(codes) && ld_codes % 16 == 0, "rows of codes must be 16-byte aligned");
     Fp8QuantArgs a = {static_cast<const uint8_t*>(x), codes, scales, (size_t)ld_x * size, (size_t)x_step * size, ld_codes, ld_scales, rows, cols,
-                      out_cols, wide, out_rows, scale_rows, blocks, 0, pow2 ? 1u : 0u};
+                      out_cols, wide, out_rows, scale_rows, blocks, 0, pow2 ? 1u : 0u, 65535u / blocks + 1};
     a.vec = aligned16(x) && a.ld_x % 16 == 0 && (batch == 1 || a.x_step % 16 == 0) ? 1u : 0u;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (type == CMX_OUT_BF16) return launch<CMX_OUT_BF16>(a, batch, fmt, square != 0, transposed != 0, s);
