@@ -507,7 +507,12 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
                 __builtin_amdgcn_sched_barrier(0);
             }
             part[x % 4] = block_product<FMT>(b[i & 1], a[j]);
+            if constexpr (FN >= 4) __builtin_amdgcn_sched_barrier(0);        // (reads in front of a product would be waited for with its own)
             if (x >= 3) add(x - 3);
+            if (x == FM + 2) {
+#pragma unroll
+                for (uint32_t l = 0; l < FM; ++l) s_next[l] = next_scales[a_row + 16 * l];
+            }
             if (i + 1 < FN) {
                 if (j == 0) b[(i + 1) & 1] = fragment(at + b_lo, i + 1);
                 if constexpr (ROW_SCALES)
@@ -517,7 +522,6 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
             } else {
                 if (j == 0) b[0] = fragment(next_at + b_lo, 0);
                 a[j] = fragment(next_at + a_lo, j);
-                s_next[j] = next_scales[a_row + 16 * j];
                 if (j < kEarly) issue(kb + SLOTS, slot, j, gone_here);
                 if constexpr (ROW_SCALES)
                     if (j == FM - 1) row_scales(next_scales, 0);
