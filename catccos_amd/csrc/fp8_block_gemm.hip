@@ -406,6 +406,8 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
                      "v"(kb <= last ? line_off : 0x80000000u), "s"(line_buf), "s"(same(kb * kBlockK)) : "memory");
     };
     // scales of blocks span * kScaleSpan .. + kScaleSpan, [block][row], into half span % 2; a thread has some rows' four blocks
+    // (fetched in a span's first block; placed at the end of a block that has another one's barrier between it and the last, where they are read first)
+    constexpr uint32_t kPlace = kScaleSpan - 3;
     constexpr uint32_t kPieces = kScaleRows * (kScaleSpan / 4), kMine = (kPieces + NT - 1) / NT;
     float staged[kMine][4];
     const auto fetch_scales = [&](uint32_t span) {
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
         }
 #pragma unroll
         for (uint32_t x = FN * FM - 3; x < FN * FM; ++x) add(x);
-        if (in_span == kScaleSpan / 2 && more) place_scales(span + 1);
+        if (in_span == kPlace && more) place_scales(span + 1);
 #pragma unroll
         for (uint32_t j = 0; j < FM; ++j) s[j] = ROW_SCALES ? s_next[j] : s_next[j] * sb;
         slot = next;

@@ -162,7 +162,11 @@ SHAPES = [(1, 1, 16), (1, 130, 128), (1, 4096, 1040), (2, 7, 112), (7, 64, 144),
           (100, 1000, 1040), (128, 128, 128), (129, 256, 2048), (300, 999, 144), (1000, 1030, 528), (2049, 520, 1168), (4101, 4105, 272), (4352, 4096, 1296)]
 
 
-@pytest.mark.parametrize("m,n,k", SHAPES)
+# sizes that take each of the kernels (few rows in tiles of 16 x 16 to 64 x 32, tiles of 128 x 128 to 256 x 256, K in parts), ragged in each axis
+WAYS = [(300, 999, 144), (30, 4100, 1040), (64, 4100, 1168), (100, 4104, 912), (90, 16388, 2064), (250, 4100, 7184), (66, 16380, 7184), (1400, 4100, 1040), (5000, 4100, 1168), (4000, 4090, 2064)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES + WAYS)
 @pytest.mark.parametrize("b_rows", [128, 1])
 @pytest.mark.parametrize("fmt", ["E4M3", "E5M2"])
 def test_gemm_of_exact_sums(m, n, k, b_rows, fmt):
@@ -257,7 +261,8 @@ def _groups(sizes, n, k, seed, fmt="E4M3", extra=0):
 
 MANY = [0] * 300 + [3, 0, 17, 1] * 20 + [0, 40] + [0] * 200 + [5]
 GROUPS = [([1], 64, 128), ([0, 0, 1, 0], 130, 144), ([3, 0, 16, 17, 1], 200, 272), ([33, 64, 0, 5], 129, 1040), ([100, 0, 200, 70], 256, 400), ([300, 1, 0, 513, 128], 384, 528), (MANY, 40, 144),
-          ([2100, 0, 2500, 1], 4100, 144), ([1] * 256, 136, 256), ([0, 0, 0], 64, 128), ([5, -3, 9], 64, 128)]
+          ([2100, 0, 2500, 1], 4100, 144), ([1] * 256, 136, 256), ([0, 0, 0], 64, 128), ([5, -3, 9], 64, 128), ([4, 6, 0, 9] * 16, 8200, 272), ([100, 130, 0, 128] * 2, 2060, 400),
+          ([2500, 10, 300, 0, 200], 4090, 2064)]
 
 
 @pytest.mark.parametrize("sizes,n,k", GROUPS)
