@@ -687,7 +687,7 @@ Plan plan_of(const Fp8GemmArgs& p, uint32_t cus, bool may_split) {
     tile(Way::kTile256x128, 256, 128, 5.0, 1.05);
     tile(Way::kTile128, 128, 128, 4.5, 0.61);
     tile(Way::kTile256, 256, 256, 6.0, 1.75);
-    if (!grouped && may_split && p.m > 16) {
+    if (!grouped && may_split && p.m > 16) {                          // (ops.py knows that fewer rows, and fewer than 8 blocks, are not split)
         const uint64_t tiles = (uint64_t)ceil_div(p.m, 128) * ceil_div(p.n, 128);
         const uint32_t splits = (uint32_t)std::min<uint64_t>({cus / std::max<uint64_t>(tiles, 1), 16, p.blocks / 4});
         if (splits > 1) {

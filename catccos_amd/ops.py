@@ -223,10 +223,14 @@ def mxfp4_gemv(x: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: str
                    (_OUT_DTYPE[out], m, n), n, OUT[out], m, n, k)
 
 
+_FP8 = {"E4M3": 0, "E5M2": 1}
+
+
 def _fp8(fmt: str) -> int:
-    if fmt not in ("E4M3", "E5M2"):
+    code = _FP8.get(fmt)
+    if code is None:
         raise ValueError("E4M3 or E5M2")
-    return FMT[fmt]
+    return code
 
 
 def fp8_block_quant(x: torch.Tensor, fmt: str = "E4M3", square: bool = False, transposed: bool = False, pow2: bool = False):
@@ -255,9 +259,10 @@ def fp8_block_quant(x: torch.Tensor, fmt: str = "E4M3", square: bool = False, tr
                    batch, rows, cols, fmt, 1 if square else 0, 1 if transposed else 0, 1 if pow2 else 0)
 
 
-def _scale_pitch(scale, rows: int, blocks: int) -> int:
-    assert scale.dtype == torch.float32 and scale.dim() == 2 and scale.shape[0] == rows and scale.shape[1] >= blocks, "scales"
-    return max(_pitch(scale, scale.shape[1]), blocks)
+def _scale_pitch(scale, shape, rows: int, blocks: int) -> int:
+    """Elements from row to row of scales [rows, >= blocks], whose shape is `shape`."""
+    assert scale.dtype == torch.float32 and len(shape) == 2 and shape[0] == rows and shape[1] >= blocks, "scales"
+    return shape[1] if scale.is_contiguous() else max(_pitch(scale, shape[1]), blocks)
 
 
 def fp8_block_gemm_workspace_bytes(m: int, n: int, k: int) -> int:
@@ -269,26 +274,26 @@ def fp8_block_gemm_workspace_bytes(m: int, n: int, k: int) -> int:
 def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16", c=None, workspace=None) -> torch.Tensor:
     """a u8 [m, k] with a_scale fp32 [m, >= ceil(k/128)] times b u8 [n, k] with b_scale [ceil(n/128), ..] (a weight's 128 x 128) or [n, ..] (1 x 128,
     as a weight's gradient has on both sides) -> c [m, n]; operands as fp8_block_quant makes them, k a multiple of 16."""
-    _here(a, a_scale, b, b_scale, c, workspace)
-    (m, k), (n, kb) = a.shape, b.shape
+    _here(a, a_scale, b, b_scale)
+    (m, k), (n, kb), of_a, of_b = a.shape, b.shape, a_scale.shape, b_scale.shape
     _fits(m | n | k)
     assert a.dtype == b.dtype == torch.uint8 and k == kb
     blocks = (k + 127) // 128
-    b_rows = 1 if n > 1 and b_scale.shape[0] == n else 128
-    ld_as, ld_bs = _scale_pitch(a_scale, m, blocks), _scale_pitch(b_scale, n if b_rows == 1 else (n + 127) // 128, blocks)
-    ldc = n
+    b_rows, of_n = (1, n) if n > 1 and of_b[0] == n else (128, (n + 127) // 128)
+    ld_as, ld_bs = _scale_pitch(a_scale, of_a, m, blocks), _scale_pitch(b_scale, of_b, of_n, blocks)
     if c is None:
-        made = (_OUT_DTYPE[out], m, n)
+        made, ldc = (_OUT_DTYPE[out], m, n), n
     else:
-        made = c
+        _here(a, c)
         assert c.shape == (m, n) and c.dtype == _OUT_DTYPE[out]
-        ldc = _pitch(c, n)
-    if m > 16 or workspace is not None:                                # (a few rows never need one)
+        made, ldc = c, _pitch(c, n)
+    if workspace is not None:
+        _here(a, workspace)
+        assert workspace.is_contiguous() and workspace.nbytes >= fp8_block_gemm_workspace_bytes(m, n, k)
+    elif m > 16 and k > 896:                                           # (others never need one)
         need = fp8_block_gemm_workspace_bytes(m, n, k)
-        if workspace is None:
-            workspace = _empty(a, torch.uint8, need) if need else None
-        else:
-            assert workspace.is_contiguous() and workspace.nbytes >= need
+        if need:
+            workspace = _empty(a, torch.uint8, need)
     got = _launch("cmx_fp8_block_gemm", a, _pitch(a, k), a_scale, ld_as, b, _pitch(b, k), b_scale, ld_bs, b_rows, made, ldc, m, n, k, _fp8(fmt), OUT[out], workspace)
     return got if c is None else c
 
@@ -296,22 +301,21 @@ def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16",
 def fp8_block_gmm(a, a_scale, b, b_scale, group_sizes, fmt: str = "E4M3", out: str = "bf16", c=None) -> torch.Tensor:
     """fp8_block_gemm for ragged groups: a u8 [m_total, k], b u8 [G, n, k] with b_scale fp32 [G, ceil(n/128), ceil(k/128)], group_sizes int32 [G] on the
     device -> [m_total, n].  Rows behind the groups are zeros in a new tensor and stay as they are in the caller's c."""
-    _here(a, a_scale, b, b_scale, group_sizes, c)
+    _here(a, a_scale, b, b_scale, group_sizes)
     (m, k), (g, n, kb) = a.shape, b.shape
     _fits(m | n | k | g)
     blocks = (k + 127) // 128
     assert a.dtype == b.dtype == torch.uint8 and k == kb and b.is_contiguous()
     assert b_scale.dtype == torch.float32 and b_scale.shape == (g, (n + 127) // 128, blocks) and b_scale.is_contiguous()
     assert group_sizes.dtype == torch.int32 and group_sizes.shape == (g,) and group_sizes.is_contiguous()
-    ldc = n
     if c is None:
-        made = (_OUT_DTYPE[out], m, n)
+        made, ldc = (_OUT_DTYPE[out], m, n), n
     else:
-        made = c
+        _here(a, c)
         assert c.shape == (m, n) and c.dtype == _OUT_DTYPE[out]
-        ldc = _pitch(c, n)
-    got = _launch("cmx_fp8_block_gmm", a, _pitch(a, k), a_scale, _scale_pitch(a_scale, m, blocks), b, b_scale, made, ldc, group_sizes, g, m, n, k, _fp8(fmt), OUT[out],
-                  1 if c is None else 0)
+        made, ldc = c, _pitch(c, n)
+    got = _launch("cmx_fp8_block_gmm", a, _pitch(a, k), a_scale, _scale_pitch(a_scale, a_scale.shape, m, blocks), b, b_scale, made, ldc, group_sizes, g, m, n, k, _fp8(fmt),
+                  OUT[out], 1 if c is None else 0)
     return got if c is None else c
 
 
