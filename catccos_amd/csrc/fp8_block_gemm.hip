@@ -480,6 +480,26 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
     };
     float sb = ROW_SCALES ? 0.0f : b_scale[0];
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((SLOTS - 2) * kLoads + kEarly) : "memory");
+    // A wavefront whose rows do not exist (a group's last tile is half empty on average) only brings its share of the operands
+    if (wm * (TM / WM) >= w.rows) {
+        uint32_t slot = 0;
+        for (uint32_t kb = 0; kb < p.blocks; ++kb) {
+            const uint32_t span = kb / kScaleSpan, in_span = kb % kScaleSpan, before = slot == 0 ? SLOTS - 1 : slot - 1;
+            const bool more = (span + 1) * kScaleSpan < p.blocks;
+            if (in_span == 0 && more) fetch_scales(span + 1);
+            if constexpr (kTouch)
+                if (wave < 2) touch(kb + kAhead);
+#pragma unroll
+            for (uint32_t l = kEarly; l < kLoads; ++l) issue(kb + SLOTS - 1, before, l, gone(kb + SLOTS - 1));
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((SLOTS - 2) * kLoads) : "memory");
+#pragma unroll
+            for (uint32_t l = 0; l < kEarly; ++l) issue(kb + SLOTS, slot, l, gone(kb + SLOTS));
+            if (in_span == kPlace && more) place_scales(span + 1);
+            slot = slot + 1 < SLOTS ? slot + 1 : 0;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        return;
+    }
     b[0] = fragment(lds0 + b_lo, 0);
     if constexpr (ROW_SCALES) row_scales(scales_of(0), 0);
 #pragma unroll

@@ -308,6 +308,8 @@ def fp8_block_gmm(a, a_scale, b, b_scale, group_sizes, fmt: str = "E4M3", out: s
     assert a.dtype == b.dtype == torch.uint8 and k == kb and b.is_contiguous()
     assert b_scale.dtype == torch.float32 and b_scale.shape == (g, (n + 127) // 128, blocks) and b_scale.is_contiguous()
     assert group_sizes.dtype == torch.int32 and group_sizes.shape == (g,) and group_sizes.is_contiguous()
+    if g == 0 and c is None:
+        return torch.zeros((m, n), dtype=_OUT_DTYPE[out], device=a.device)
     if c is None:
         made, ldc = (_OUT_DTYPE[out], m, n), n
     else:

@@ -290,6 +290,17 @@ def test_gmm_of_sizes_that_add_up_to_more_than_there_are():
     assert torch.equal(ops.fp8_block_gmm(a, sa, b, sb, counts, out="fp32").double(), want[:35])
 
 
+def test_products_of_nothing():
+    from catccos_amd import ops
+    u, f = lambda *s: torch.zeros(s, dtype=torch.uint8, device="cuda"), lambda *s: torch.ones(s, device="cuda")
+    assert ops.fp8_block_gemm(u(0, 128), f(0, 1), u(8, 128), f(1, 1)).shape == (0, 8) and ops.fp8_block_gemm(u(5, 128), f(5, 1), u(0, 128), f(0, 1)).shape == (5, 0)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert not bool(ops.fp8_block_gmm(u(5, 128), f(5, 1), u(0, 8, 128), f(0, 1, 1), none).any())
+    c = torch.full((5, 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert bool((ops.fp8_block_gmm(u(5, 128), f(5, 1), u(0, 8, 128), f(0, 1, 1), none, c=c) == 7).all())
+    assert ops.fp8_block_gmm(u(0, 128), f(0, 1), u(2, 8, 128), f(2, 1, 1), torch.zeros(2, dtype=torch.int32, device="cuda")).shape == (0, 8)
+
+
 def test_equal_calls_give_equal_bits():
     from catccos_amd import ops
     g = torch.Generator(device="cuda").manual_seed(1)
