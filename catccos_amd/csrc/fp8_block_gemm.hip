@@ -193,8 +193,12 @@ __device__ __forceinline__ uint32_t place_of(uint32_t row, uint32_t piece) { ret
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------
 // A workgroup owns 16 FN columns of c and 16 FM rows over all of K; its wavefronts take the blocks of K in turn, DEPTH of each in flight, and join their
-// sums in LDS in the order of the wavefronts.  Loads take whole
-// lines (8 rows of 128 bytes); lane l of a fragment holds row l % 16, the 16-byte pieces l / 16 and l / 16 + 4 of a block, so operands change lanes through the LDS.
+// sums in LDS in the order of the wavefronts.  Loads take whole lines (8 rows of 128 bytes); lane l of a fragment holds row l % 16, the 16-byte pieces l / 16 and l / 16 + 4
+// of a block, so operands change lanes through the LDS (loads as fragments want them, 16 rows of 64 bytes, cost the vector cache twice as much: 16 rows of 4096 x 7168
+// 10.7 us, so 8.2; 64 rows 18.3, so 12.6).
+// Bound by reading the weights where rows are few: one row of 4096 x 7168 in 7.3 us (4.0 TB/s, 2.5 of it the launch), 256 rows on 256 experts of 7168 x 2048 in 400 us (5.9 TB/s);
+// by operands through the vector cache where they are more: 64 rows of 4096 x 7168 pull 458 KB into each CU in 12.8 us.  Deeper rings change nothing (64 rows: 2 blocks 12.6, 3 13.1,
+// 4 13.6).
 template <int FMT, int FN, int FM, int DEPTH, bool ROW_SCALES>
 __global__ __launch_bounds__(FN * FM == 1 ? 1024 : 512) void fp8_rows_kernel(const Fp8GemmArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -331,6 +335,10 @@ __global__ __launch_bounds__(FN * FM == 1 ? 1024 : 512) void fp8_rows_kernel(con
 
 // ---- tiles through the LDS -------------------------------------------------------------------------------------------------
 // A workgroup of WN x WM wavefronts owns TN columns and TM rows of c.  Blocks of K travel by LDS-DMA into SLOTS slots.
+// Two wavefronts to a SIMD share the matrix pipe and the vector unit: products and multiply-adds alone, without memory, run at 3.84 PFLOP/s (32 x 32 x 64 products: 3.36).  A
+// wavefront's 128 x 64 of c are 128 accumulators; 128 x 128 would not leave the vector unit a register.  256 x 256 tiles, 8192 x 4096 x 7168: 210 - 220 us (2.2 PFLOP/s), the matrix
+// pipe busy for 47 - 53 % of a clock that the chip lowers to 1.8 - 2.2 GHz under it.  Of 217 us at an earlier step, without the multiply-adds 202, without the loads of operands 174,
+// without the reads of b from the LDS 208.  With a scale for each row of b twice the vector work: 4096 x 2048 x 2784 36 us (28 with one for 128 rows).
 __device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ void dma16(uint32_t lds, uint32_t off, v4i rsrc, uint32_t soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(same(lds)), "v"(off), "s"(rsrc), "s"(same(soff)) : "memory");

@@ -193,7 +193,8 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const Fp8QuantArgs 
 }
 
 // Tiles of 128 x 128 of x: blocks of 128 x 128, and both kinds of the transpose.  A thread holds 8 x 8 elements; what is turned passes through the LDS
-// as codes, so that both sides of memory see whole lines.
+// as codes, so that both sides of memory see whole lines.  2777 x 4096 bf16, transposed: 10.6 us, of which the launch takes 2.5 and the bytes 6.6; 8192 x 7168 45 us, in
+// blocks of 128 x 128 39 (past the caches 47 and 42: these stay in them).
 template <int TYPE, int FMT, bool SQUARE, bool TURNED>
 __global__ __launch_bounds__(256) void fp8_quant_tile_kernel(const Fp8QuantArgs a) {
     static_assert(SQUARE || TURNED, "rows of x itself have a kernel of their own");
