@@ -771,7 +771,7 @@ int check_product(const Fp8GemmArgs& p, const void* c, int fmt) {
 
 int cmx::preload_fp8_gemm_kernels() {
     hipFuncAttributes attr;
-    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::fp8_rows_kernel<CMX_FMT_E4M3, 1, 1, 4, false>)));
+    CMX_HIP(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(cmx::fp8_rows_kernel<CMX_FMT_E4M3, 1, 1, 2, false>)));
     return CMX_OK;
 }
 
