@@ -540,15 +540,17 @@ def quant_scatter(x: torch.Tensor, src2sorted: torch.Tensor, top_k: int, packed:
 
 
 def moe_token_unpermute(y: torch.Tensor, src2sorted: torch.Tensor, probs: torch.Tensor) -> torch.Tensor:
-    """y bf16 [rows, h]; probs fp32 [T, topK] -> bf16 [T, h]."""
-    _need_cuda(y, src2sorted, probs)
+    """y bf16 [rows, h]; src2sorted int32 [T * topK]; probs fp32 [T, topK] -> bf16 [T, h]."""
+    assert _TYPE.get(y.dtype) == 0, "rows in bf16"
     assert probs.dtype == torch.float32 and probs.is_contiguous()
     t, top_k = probs.shape
     rows, h = y.shape
+    assert _routes(src2sorted, top_k) == t
+    pitch = _pitch(y, h)
+    _need_cuda(y, src2sorted, probs)
     out = torch.empty((t, h), dtype=y.dtype, device=y.device)
     lib = _lib.load()
-    _lib.check(lib.cmx_moe_token_unpermute(_p(y), y.stride(0), rows, _p(src2sorted), _p(probs), _p(out), h, t, h, top_k,
-                                           _stream()))
+    _lib.check(lib.cmx_moe_token_unpermute(_p(y), pitch, rows, _p(src2sorted), _p(probs), _p(out), h, t, h, top_k, _stream()))
     return out
 
 
@@ -586,7 +588,8 @@ def moe_token_permute_grad(dy: torch.Tensor, src2sorted: torch.Tensor, top_k: in
 
 def moe_token_unpermute_grad(dout: torch.Tensor, y: torch.Tensor, src2sorted: torch.Tensor, probs: torch.Tensor):
     """Gradients of moe_token_unpermute(y, src2sorted, probs): dout [T, h] and y [rows, h] bf16 / fp16 / fp32, probs fp32 [T, top_k] -> (dy [rows, h],
-    dprobs fp32 [T, top_k]).  Rows of no route get zeros, dropped routes a zero."""
+    dprobs fp32 [T, top_k]).  Rows of no route get zeros, dropped routes a zero.  (moe_token_unpermute itself
+    takes bf16 rows only.)"""
     _here(dout, y, src2sorted, probs)
     (t, h), (rows, hy), top_k = dout.shape, y.shape, probs.shape[1]
     _fits(t | h | rows | top_k)

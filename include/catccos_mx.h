@@ -445,7 +445,7 @@ int cmx_quant_scatter_zeroed(const void* x, uint32_t ld_x, const int32_t* src2so
  * Weighted top-k combine.  Replaces KernelMoeTokenUnpermute<bf16,int32,float,true>
  * (examples/aux_ops/moe_token_unpermute/moe_token_unpermute.h:233-366):
  * out[t] = bf16( sum_k probs[t,k] * y[src2sorted[t*top_k+k]] ), fp32 multiply then fp32 add in k
- * order; indices outside [0, rows) contribute nothing.
+ * order; indices outside [0, rows) contribute nothing.  y and out are bf16, their rows 16-byte aligned.
  * ---------------------------------------------------------------------------------------- */
 int cmx_moe_token_unpermute(const void* y, uint32_t ld_y, uint32_t rows, const int32_t* src2sorted,
                             const float* probs, void* out, uint32_t ld_out, uint32_t tokens, uint32_t hidden,
@@ -457,7 +457,8 @@ int cmx_moe_token_unpermute(const void* y, uint32_t ld_y, uint32_t rows, const i
  *   permute         out[dst(t, r)] = x[t]                        rows of any elements of 1, 2 or 4 bytes, codes and scales among them
  *   permute_grad    dx[t] = sum_r dy[dst(t, r)]                  of `type` (CMX_OUT_BF16 / FP16 / FP32), in fp32 in the order of r, rounded once
  *   unpermute_grad  of cmx_moe_token_unpermute(y, probs): dy[dst(t, r)] = probs[t, r] * dout[t] in fp32, rounded once; dprobs[t, r] = sum_h
- *                   dout[t, h] * y[dst(t, r), h] in fp32, zero for a dropped route (dprobs fp32 [tokens, top_k])
+ *                   dout[t, h] * y[dst(t, r), h] in fp32, zero for a dropped route (dprobs fp32 [tokens, top_k]).  dout, y and dy of `type`: also
+ *                   those in which cmx_moe_token_unpermute, bf16 only, does not read y
  * Rows of out and dy (`rows` of them) that no route is sent to are left as they were, or cleared with zero_rest.  Pitches in elements; elements' alignment.  No
  * input may overlap an output.  top_k <= 64, tokens * top_k and rows < 2^31.
  * ---------------------------------------------------------------------------------------- */
