@@ -273,11 +273,12 @@ def fp8_block_gemm_workspace_bytes(m: int, n: int, k: int) -> int:
 
 def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16", c=None, workspace=None) -> torch.Tensor:
     """a u8 [m, k] with a_scale fp32 [m, >= ceil(k/128)] times b u8 [n, k] with b_scale [ceil(n/128), ..] (a weight's 128 x 128) or [n, ..] (1 x 128,
-    as a weight's gradient has on both sides) -> c [m, n]; operands as fp8_block_quant makes them, k a multiple of 16."""
+    as a weight's gradient has on both sides) -> c [m, n]; operands as fp8_block_quant makes them, k a multiple of 16 (zeros where it is 0)."""
     _here(a, a_scale, b, b_scale)
     (m, k), (n, kb), of_a, of_b = a.shape, b.shape, a_scale.shape, b_scale.shape
     _fits(m | n | k)
     assert a.dtype == b.dtype == torch.uint8 and k == kb
+    fmt = _fp8(fmt)
     blocks = (k + 127) // 128
     b_rows, of_n = (1, n) if n > 1 and of_b[0] == n else (128, (n + 127) // 128)
     ld_as, ld_bs = _scale_pitch(a_scale, of_a, m, blocks), _scale_pitch(b_scale, of_b, of_n, blocks)
@@ -290,11 +291,13 @@ def fp8_block_gemm(a, a_scale, b, b_scale, fmt: str = "E4M3", out: str = "bf16",
     if workspace is not None:
         _here(a, workspace)
         assert workspace.is_contiguous() and workspace.nbytes >= fp8_block_gemm_workspace_bytes(m, n, k)
-    elif m > 16 and k > 896:                                           # (others never need one)
+    if k == 0:                                                         # (sums of nothing: the gradient of the weight of an expert without rows)
+        return torch.zeros((m, n), dtype=_OUT_DTYPE[out], device=a.device) if c is None else c.zero_()
+    if workspace is None and m > 16 and k > 896:                       # (others never need one)
         need = fp8_block_gemm_workspace_bytes(m, n, k)
         if need:
             workspace = _empty(a, torch.uint8, need)
-    got = _launch("cmx_fp8_block_gemm", a, _pitch(a, k), a_scale, ld_as, b, _pitch(b, k), b_scale, ld_bs, b_rows, made, ldc, m, n, k, _fp8(fmt), OUT[out], workspace)
+    got = _launch("cmx_fp8_block_gemm", a, _pitch(a, k), a_scale, ld_as, b, _pitch(b, k), b_scale, ld_bs, b_rows, made, ldc, m, n, k, fmt, OUT[out], workspace)
     return got if c is None else c
 
 
@@ -310,13 +313,17 @@ def fp8_block_gmm(a, a_scale, b, b_scale, group_sizes, fmt: str = "E4M3", out: s
     assert group_sizes.dtype == torch.int32 and group_sizes.shape == (g,) and group_sizes.is_contiguous()
     if g == 0 and c is None:
         return torch.zeros((m, n), dtype=_OUT_DTYPE[out], device=a.device)
+    ld_as = _scale_pitch(a_scale, a_scale.shape, m, blocks)
+    if k == 0:                                                         # sums of nothing: those of a piece of zeros, in the rows of groups only
+        new = lambda t, *shape: torch.zeros(shape, dtype=t.dtype, device=t.device)
+        return fp8_block_gmm(new(a, m, 16), new(a_scale, m, 1), new(b, g, n, 16), new(b_scale, g, (n + 127) // 128, 1), group_sizes, fmt, out, c)
     if c is None:
         made, ldc = (_OUT_DTYPE[out], m, n), n
     else:
         _here(a, c)
         assert c.shape == (m, n) and c.dtype == _OUT_DTYPE[out]
         made, ldc = c, _pitch(c, n)
-    got = _launch("cmx_fp8_block_gmm", a, _pitch(a, k), a_scale, _scale_pitch(a_scale, a_scale.shape, m, blocks), b, b_scale, made, ldc, group_sizes, g, m, n, k, _fp8(fmt),
+    got = _launch("cmx_fp8_block_gmm", a, _pitch(a, k), a_scale, ld_as, b, b_scale, made, ldc, group_sizes, g, m, n, k, _fp8(fmt),
                   OUT[out], 1 if c is None else 0)
     return got if c is None else c
 

@@ -210,7 +210,7 @@ int cmx_mx_gmm(const uint8_t* a, uint32_t lda, const uint8_t* a_scale, uint32_t 
  *
  * cmx_fp8_block_gmm    the same over ragged groups of rows, as cmx_mx_gmm has them: group_sizes int32 [groups] on the device; b [groups, n, k] and
  *   b_scale [groups, ceil(n / 128), ceil(k / 128)] dense.  Rows behind the groups, up to m_total, are left untouched, or cleared with zero_rest.  No workspace.
- * k a multiple of 16; operand rows 16-byte aligned, at most 2^22 bytes apart.
+ * k a positive multiple of 16; operand rows 16-byte aligned, at most 2^22 bytes apart.
  * ---------------------------------------------------------------------------------------- */
 int cmx_fp8_block_quant(const void* x, uint32_t ld_x, uint64_t x_step, int type, uint8_t* codes, uint32_t ld_codes, float* scales,
                         uint32_t ld_scales, uint32_t batch, uint32_t rows, uint32_t cols, int fmt, int square, int transposed, int pow2,
