@@ -775,6 +775,23 @@ int cmx::preload_fp8_gemm_kernels() {
     return CMX_OK;
 }
 
+#ifdef CMX_TEST_HOOKS
+// the way of a product on a chip of `cus` CUs: Way, and 256 times its parts of K; groups = 0: dense
+extern "C" int cmx_debug_fp8_way(uint32_t m, uint32_t n, uint32_t k, uint32_t groups, int workspace, uint32_t cus) {
+    using namespace cmx;
+    const int32_t sizes = 0;
+    Fp8GemmArgs p{};
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.blocks = ceil_div(k, kBlockK);
+    p.groups = groups;
+    p.sizes = groups != 0 ? &sizes : nullptr;
+    const Plan plan = plan_of(p, cus, workspace != 0);
+    return (int)plan.way | (int)plan.splits << 8;
+}
+#endif
+
 extern "C" size_t cmx_fp8_block_gemm_workspace_bytes(uint32_t m, uint32_t n, uint32_t k) {
     using namespace cmx;
     if (m == 0 || n == 0 || k == 0) return 0;

@@ -45,6 +45,7 @@ _HOOKS = {
     "cmx_debug_disable_streaming": (_C.c_int, [_C.c_int]),
     "cmx_debug_pretiled_tile_rows": (_C.c_int, [_C.c_int]),
     "cmx_debug_force_ksplit": (_C.c_int, [_C.c_int] * 3),
+    "cmx_debug_fp8_way": (_C.c_int, [_C.c_uint32] * 4 + [_C.c_int, _C.c_uint32]),
 }
 _test_lib = None
 
