@@ -191,6 +191,13 @@ __device__ __forceinline__ void static_for(F&& f) {
 // Rows of 128 bytes in LDS: row r holds its 16-byte piece p at place p ^ (r / 2 % 8), so that the 16 rows that a fragment reads at a time lie in different banks
 __device__ __forceinline__ uint32_t place_of(uint32_t row, uint32_t piece) { return piece ^ ((row >> 1) & 7u); }
 
+// Between LDS writes of some lanes and reads of the same wavefront's others, or the other way round: the LDS takes a wavefront's accesses in order, so only the compiler, which
+// sees one lane, has to keep them so.  No instruction
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- few rows ------------------------------------------------------------------------------------------------------------
 // A workgroup owns 16 FN columns of c and 16 FM rows over all of K; its wavefronts take the blocks of K in turn, DEPTH of each in flight, and join their
 // sums in LDS in the order of the wavefronts.  Loads take whole lines (8 rows of 128 bytes); lane l of a fragment holds row l % 16, the 16-byte pieces l / 16 and l / 16 + 4
@@ -259,7 +266,9 @@ __global__ __launch_bounds__(FN * FM == 1 ? 1024 : 512) void fp8_rows_kernel(con
             if (clear) v[h] = (v4i){0, 0, 0, 0};
             *reinterpret_cast<v4i*>(at + put + h * (8 * kBlockK) + 16 * place_of(8 * h + row8, piece)) = v[h];
         }
+        wave_fence();
         const v4i lo = *reinterpret_cast<const v4i*>(at + get), hi = *reinterpret_cast<const v4i*>(at + (get ^ 64u));
+        wave_fence();
         return (v8i){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
     v4i b[DEPTH][FN][2], a[DEPTH][FM][2];
