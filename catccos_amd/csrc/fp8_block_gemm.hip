@@ -204,8 +204,8 @@ __device__ __forceinline__ void wave_fence() {
 // of a block, so operands change lanes through the LDS (loads as fragments want them, 16 rows of 64 bytes, cost the vector cache twice as much: 16 rows of 4096 x 7168
 // 10.7 us, so 8.2; 64 rows 18.3, so 12.6).
 // Bound by reading the weights where rows are few: one row of 4096 x 7168 in 7.3 us (4.0 TB/s, 2.5 of it the launch), 256 rows on 256 experts of 7168 x 2048 in 400 us (5.9 TB/s);
-// by operands through the vector cache where they are more: 64 rows of 4096 x 7168 pull 458 KB into each CU in 12.8 us.  Deeper rings change nothing (64 rows: 2 blocks 12.6, 3 13.1,
-// 4 13.6).
+// by loads of operands where they are more: 64 rows of 4096 x 7168 pull 458 KB into each CU in 12.9 us, of which loads alone take 11.9 (half of them weights that two XCDs fetch each for
+// itself: the row tiles of the same columns are neighbours in number).  Deeper rings change nothing (64 rows: 2 blocks 12.6, 3 13.1, 4 13.6).
 template <int FMT, int FN, int FM, int DEPTH, bool ROW_SCALES>
 __global__ __launch_bounds__(FN * FM == 1 ? 1024 : 512) void fp8_rows_kernel(const Fp8GemmArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -345,9 +345,10 @@ __global__ __launch_bounds__(FN * FM == 1 ? 1024 : 512) void fp8_rows_kernel(con
 // ---- tiles through the LDS -------------------------------------------------------------------------------------------------
 // A workgroup of WN x WM wavefronts owns TN columns and TM rows of c.  Blocks of K travel by LDS-DMA into SLOTS slots.
 // Two wavefronts to a SIMD share the matrix pipe and the vector unit: products and multiply-adds alone, without memory, run at 3.84 PFLOP/s (32 x 32 x 64 products: 3.36).  A
-// wavefront's 128 x 64 of c are 128 accumulators; 128 x 128 would not leave the vector unit a register.  256 x 256 tiles, 8192 x 4096 x 7168: 210 - 220 us (2.2 PFLOP/s), the matrix
-// pipe busy for 47 - 53 % of a clock that the chip lowers to 1.8 - 2.2 GHz under it.  Of 217 us at an earlier step, without the multiply-adds 202, without the loads of operands 174,
-// without the reads of b from the LDS 208.  With a scale for each row of b twice the vector work: 4096 x 2048 x 2784 36 us (28 with one for 128 rows).
+// wavefront's 128 x 64 of c are 128 accumulators; 128 x 128 would not leave the vector unit a register.  256 x 256 tiles, 8192 x 4096 x 7168: 216 - 224 us (2.2 PFLOP/s), the matrix
+// pipe busy for 47 - 53 % of a clock that the chip lowers to 1.8 - 2.2 GHz under it.  Of 231 us in one run of it, without the multiply-adds 199, without the loads of operands 172,
+// without both 156.  With a scale for each row of b twice the vector work: 4096 x 2048 x 2784 37 us (31 with one for 128 rows), a block of K 1.37: 0.27 of it waits for loads, 0.43 are
+// multiply-adds (0.24 the products of scales), 0.66 products, barriers and LDS reads; they add up, and no unit is full (matrix pipe 23 %, vector unit 30 %).
 __device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ void dma16(uint32_t lds, uint32_t off, v4i rsrc, uint32_t soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(same(lds)), "v"(off), "s"(rsrc), "s"(same(soff)) : "memory");
@@ -411,7 +412,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(const Fp8GemmArg
     };
     // Two slots: a block's loads have less than a block's time, so lines that are not in the L2 by then stop everybody.  Of the workgroups that work on the same rows
     // of an operand at the same time (8 x 4 tiles on an XCD, as locate numbers them) each asks for a share of the lines of a later block, a dword of each, into LDS
-    // that nobody reads (16 experts of 32768 rows 955 -> 910 us; all lines by every workgroup 1056; with three slots nothing is gained).
+    // that nobody reads (16 experts of 32768 rows 955 -> 910 us in one run, all lines by every workgroup 1056; runs of the kernel as it is differ from 940 to 978; with three slots nothing is gained).
     constexpr bool kTouch = SLOTS == 2;
     constexpr uint32_t kAhead = 3;
     const uint32_t in_band = (w.row0 / TM) % 8, in_chunk = w.n_tile % 4;
@@ -684,6 +685,8 @@ struct Plan {
 //   tile 128 x 128               4.5 + 0.61                          1024 x 4096: 38.4 (56); in 256 x 128: 54
 //   tile 256 x 128               5 + 1.05                            2048 x 4096: 59.6 (56); in 128 x 128: 77, in 256 x 256: 84
 //   tile 256 x 256               6 + 1.75                            8192 x 4096: 210 (56, two rounds); in 256 x 128: 243
+// Both sides of a border are from one run; other runs are up to a tenth longer (8192 x 4096 x 7168 216 - 224).  All with a scale for 128 rows of b: with one for every row the same rule holds, for
+// which no borders were measured (4096 x 2048 x 2784 then takes a fifth longer, 64 x 4096 x 7168 a tenth).
 // Workgroups of the rows kernel follow each other without a gap, those of the tiles come in rounds.  A tile's K is split over workgroups where there are few: 3 us for
 // the launch that joins them, and twice their sums' way through memory (256 x 4096 x 7168 four ways 21, in one piece 41, by rows of 32 x 64 31).  Groups whose rows fit one tile are bound by their
 // weights, which rows of 64 x 16 read at 0.9 of a stream's rate and the tiles

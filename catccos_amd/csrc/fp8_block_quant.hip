@@ -107,7 +107,7 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
     return cvt_pk_e4m3(c, d, w, true);
 }
 
-// z into numbers that the hardware's cast rounds to the codes of the exact z / s.  Codes and the borders between them have at most 4 significant bits (E5M2 3): b is the value
+// z into numbers that the hardware's cast rounds to the codes of the exact z / s.  Codes and the borders between them have at most 5 significant bits (E5M2 4): b is the value
 // of so many bits that z * (1 / s) is next to, and if z / s is not b it lies on the side of b that the sign of z - b * s says, one fused multiply-add; the cast gets b
 // moved to that side by 2^-10 of itself, which crosses nothing.  (z - b * s is a multiple of 2^-28 of z, so that 2^30 times it exceeds the 2^-10.)
 // 8 operations an element for all of them: a look for values next to a border first takes 5, but of bf16 elements so many lie on one (3/4 and 3/2 of a maximum are borders) that

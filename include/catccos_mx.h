@@ -460,7 +460,10 @@ int cmx_moe_token_unpermute(const void* y, uint32_t ld_y, uint32_t rows, const i
  *                   dout[t, h] * y[dst(t, r), h] in fp32, zero for a dropped route (dprobs fp32 [tokens, top_k]).  dout, y and dy of `type`: also
  *                   those in which cmx_moe_token_unpermute, bf16 only, does not read y
  * Rows of out and dy (`rows` of them) that no route is sent to are left as they were, or cleared with zero_rest.  Pitches in elements; elements' alignment.  No
- * input may overlap an output.  top_k <= 64, tokens * top_k and rows < 2^31.
+ * input may overlap an output.  top_k <= 64, tokens * top_k and rows < 2^31.  A launch has fewer than 2^32 threads, or the call is refused: permute takes one for
+ * each piece of a row of x, the widest of 16, 8, 4, 2 or 1 bytes that base addresses, pitches and the row's length are multiples of, and its gradient one for
+ * each 16 bytes of dx, or for each element where these are not all multiples of 16; unpermute_grad takes 256 for each eight routes of a token (2^24 tokens of up to eight
+ * routes).  Rows of whole 16-byte pieces are the fast ones.
  * ---------------------------------------------------------------------------------------- */
 int cmx_moe_token_permute(const void* x, uint32_t ld_x, const int32_t* src2sorted, void* out, uint32_t ld_out, uint32_t rows,
                           uint32_t tokens, uint32_t hidden, uint32_t top_k, uint32_t element_bytes, int zero_rest,
